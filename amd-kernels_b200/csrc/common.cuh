@@ -229,4 +229,11 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// NaN-propagating maximum (fmaxf would drop a NaN).
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 }  // namespace hkb

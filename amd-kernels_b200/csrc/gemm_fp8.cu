@@ -21,6 +21,7 @@
 //
 // Every mbarrier wait is bounded (tc_common.cuh): on a timeout the CTA records an error bit in
 // the device status word (read by hkb_check_status), stops issuing work, and still frees TMEM.
+#include "activation.cuh"
 #include "tc_common.cuh"
 
 #include <cstdlib>
@@ -91,7 +92,7 @@ struct GemmParams {
     int a_box_rows;            // rows of A that TMA actually fetches per tile (<= BM)
     const float* sa;           // pts: [batch, M]      blockscale: [M, K/128]
     const float* sb;           // pts: [batch, N]      blockscale: [K/128, N/gn]
-    const __nv_bfloat16* bias; // pts only: [batch, N] or null
+    const __nv_bfloat16* bias; // [batch, N] or null (block scales: kOut == 5 only)
     __nv_bfloat16* C;          // [batch, M, N]
     int gn;                    // blockscale: 1 or 128
     const __nv_bfloat16* c_a;  // blockscale only: fused epilogue C = c_a * gemm + c_b, both [M, N]; null = plain
@@ -110,6 +111,10 @@ struct GemmParams {
     uint32_t* status;
     uint64_t wait_ns;          // limit of every mbarrier wait (kWaitLimitNs in production)
     int skip_kblock;           // >= 0: the producer leaves this K block of its first tile unloaded (wait-limit probe only)
+    const __nv_bfloat16* residual;   // kOut == 5: C = act(gemm + bias) + residual, [batch, M, N] or null
+    int act;                   // kOut == 5, 6: HKB_ACT_*
+    uint8_t* q_out;            // kOut == 6: codes [M, N/2] and scales [M, N/256] instead of C, or null
+    float* q_scale;
     unsigned long long* trace; // timeline build (kOut == 4) only: [grid][kTraceEvents][kTraceKb] SM clock readings
 };
 
@@ -193,6 +198,38 @@ __device__ __forceinline__ void mul_add_cols(const __nv_bfloat16* c_a, const __n
     }
 }
 
+// Bias / activation / residual epilogue on NV consecutive columns of one row from `col` (a multiple of 8, all in range or, per 8
+// columns, all out).  load_residual() goes first, ahead of every store: C may be the residual, so the compiler cannot move the
+// loads up, and they are the one long latency of the epilogue.  Plain loads for the same reason.
+template <int NV>
+__device__ __forceinline__ void load_residual(const __nv_bfloat16* rrow, int col, int N, uint4 (&r)[NV / 8]) {
+#pragma unroll
+    for (int j = 0; j < NV / 8; ++j) {
+        r[j] = make_uint4(0, 0, 0, 0);
+        if (rrow && col + 8 * j < N) r[j] = *reinterpret_cast<const uint4*>(rrow + col + 8 * j);
+    }
+}
+template <int NV>
+__device__ __forceinline__ void add_bias(const __nv_bfloat16* bias, int col, int N, float* v) {
+#pragma unroll
+    for (int j = 0; j < NV; j += 8) {
+        float b[8];
+        unpack8(col + j < N ? __ldg(reinterpret_cast<const uint4*>(bias + col + j)) : make_uint4(0, 0, 0, 0), b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j + i] += b[i];
+    }
+}
+template <int NV>
+__device__ __forceinline__ void add_residual(const uint4* r, float* v) {
+#pragma unroll
+    for (int j = 0; j < NV / 8; ++j) {
+        float f[8];
+        unpack8(r[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * j + i] += f[i];
+    }
+}
+
 // Split-cat epilogue: where 16 consecutive result columns starting at `col` (a multiple of 16; s1, s2 and
 // s3 are multiples of 16, so a chunk never straddles a boundary) of row `row` go.
 __device__ __forceinline__ __nv_bfloat16* split_cat_ptr(const GemmParams& p, int row, int col) {
@@ -237,21 +274,35 @@ __device__ __forceinline__ float2 ffma2(uint32_t a0, uint32_t a1, float2 s, floa
     return __ffma2_rn(make_float2(__uint_as_float(a0), __uint_as_float(a1)), s, c);
 }
 
+// Shared memory behind the scales.  kOut == 1: 32 rows x 128 bytes per epilogue warp.  kOut == 6: the up projection's weight scales
+// (as many as the gate's), row maxima of the eight epilogue warps for two tiles, four barriers for each of the two.
+constexpr int kGatedSbBytes = 2 * 8 * 32 * 4, kGatedMaxBytes = 2 * 8 * 32 * 4;
+template <int BN, int kOut>
+constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 : kOut == 6 ? kGatedSbBytes + kGatedMaxBytes + 8 * 8 : 0; }
+
 // kOut (block-scale): 0 = plain [M, N] result; 1 = the result also goes to p.n_peer further destinations
 // (the other GPUs' copies of the assembled output; 128-column weight-scale groups only); 2 = split-cat;
 // 3 = grouped (MoE): the M tiles come from a device-side list (expert, block), weights, weight scales and the
 // fp32 bias are per expert, rows of A / C are sorted by expert (128-column weight-scale groups only);
 // 4 = plain result plus the hand-off timeline in p.trace (diagnostic build, same code otherwise).
+// kOut (both scale schemes): 5 = bias, activation and residual: C = act(gemm + bias) + residual.
+// kOut (block-scale, 128-column weight-scale groups): 6 = gated: the BN rows of a B tile are BN/2 gate rows and the BN/2 up rows of
+// the same output columns (two boxes, no re-ordering of the weights), and the tile gives BN/2 columns act(gate) * up.  A thread
+// promotes 64 gate and the 64 matching up columns, so the product needs nobody else; with FP8 output the two warps of a row
+// exchange one maximum through shared memory (BN = 256: a tile is exactly one 128-column scale group of the result).
 template <int BN, int STAGES, bool kBlockScale, bool kGn128, bool kPair = false, int AROWS = BM, int kOut = 0>
 __global__ void __launch_bounds__(gemm_threads<BN, kBlockScale, kPair>(), 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p,
                 const __grid_constant__ CUtensorMap tmBHalf) {
     constexpr int EPI_GROUPS = (BN == 256) ? 2 : 1;     // groups of 4 warps; each owns BN/EPI_GROUPS columns
     constexpr int kScaleChunk = kOut == 1 ? 16 : 32;
-    constexpr int kStageOut = kOut == 1 ? 4 * EPI_GROUPS * 4096 : 0;       // 32 rows x 128 bytes per epilogue warp
+    constexpr int kStageOut = stage_out_bytes<BN, kOut>();
     using L = SmemLayout<BN, STAGES, kPair, AROWS, (kBlockScale && kGn128) ? 128 * EPI_GROUPS : 0, kScaleChunk, kStageOut>;
     constexpr bool kGrouped = kOut == 3;
     constexpr bool kTrace = kOut == 4;
+    constexpr bool kEpi = kOut == 5;
+    constexpr bool kGated = kOut == 6;
+    static_assert(!kGated || (kBlockScale && kGn128 && !kPair), "gated mode: block scales, 128-column groups, one CTA");
     static_assert(!kGrouped || (kBlockScale && kGn128 && !kPair), "grouped mode: block scales, 128-column groups, one CTA");
     static_assert(!kPair || BN == 256, "CTA pairs work on 256 x 256 tiles");
     constexpr int EPI_WARPS = 4 * EPI_GROUPS;
@@ -271,6 +322,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
     auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
     auto relay_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 4 + a); };
+    auto max_bar = [&](int i) { return smem_base + L::kStageOutOffset + kGatedSbBytes + kGatedMaxBytes + 8u * i; };    // gated: [tile parity][lane quarter]
     // CTA pairs with block scales: the eight epilogue warps of a CTA release a TMEM buffer on a local barrier and
     // warp 2 forwards ONE arrive per CTA to the leader's barrier, instead of sixteen arrives crossing the cluster
     constexpr bool kRelay = kPair && kBlockScale;
@@ -310,6 +362,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             mbar_init(tempty_bar(a), kRelay ? 2 : kPair ? 2 * EPI_WARPS : EPI_WARPS);   // the leader hears both CTAs' epilogues
             mbar_init(relay_bar(a), EPI_WARPS);
         }
+        if constexpr (kGated)
+            for (int i = 0; i < 8; ++i) mbar_init(max_bar(i), 2);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -370,7 +424,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     } else {
                         mbar_arrive_expect_tx(full_bar(s), stage_tx);
                         tma_load_3d(sa, &tmA, full_bar(s), kb * BK, a_row, a_z);
-                        tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), kb * BK, nb * BN, b_z);
+                        if constexpr (kGated) {
+                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), kb * BK, nb * (BN / 2), 0);
+                            tma_load_3d(sa + L::kABytes + BN / 2 * BK, &tmB, full_bar(s), kb * BK, p.N / 2 + nb * (BN / 2), 0);
+                        } else {
+                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), kb * BK, nb * BN, b_z);
+                        }
                     }
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
@@ -470,7 +529,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         constexpr int EPI_THREADS = 32 * EPI_WARPS;
         float4* const sa_slots = reinterpret_cast<float4*>(smem + L::kScaleOffset) + (threadIdx.x - EPI_WARP0 * 32);
         float* const sb_slots = reinterpret_cast<float*>(smem + L::kScaleOffset + L::kSaBytes) + ew * kScaleChunk;
+        float* const sbu_slots = reinterpret_cast<float*>(smem + L::kStageOutOffset) + ew * kScaleChunk;      // gated: the up projection's
         int sbuf = 0;
+        uint32_t max_n = 0;                      // gated: tiles whose row maxima were exchanged
         // cp.async the scales of (tile, chunk) into buffer `buf`: this thread's row of a_scale as
         // float4 slots [kb/4][thread], and lane l of each warp the weight scale of K block l of the
         // warp's column group.  Completion is awaited by the same thread (sa) / warp (sb) only.
@@ -502,11 +563,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 }
             }
             const int nsb = p.N / 128;
-            const int cg = min((tnb * BN + grp * COLS_PER_GROUP) / 128, nsb - 1);
+            const int cg = kGated ? tnb * (BN / 2) / 128 : min((tnb * BN + grp * COLS_PER_GROUP) / 128, nsb - 1);
             const int kb = kb0 + lane;
-            if (lane < kScaleChunk && kb < kblocks)
+            if (lane < kScaleChunk && kb < kblocks) {
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
                              ::"r"(smem_u32(sb_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)kb * nsb + cg) : "memory");
+                if constexpr (kGated)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                                 ::"r"(smem_u32(sbu_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)kb * nsb + nsb / 2 + cg) : "memory");
+            }
         };
         // grouped mode: the first tile at or after `t` (in this CTA's walk) that the tile list does not mark as empty
         auto next_live_tile = [&](int t) {
@@ -542,6 +607,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const int cols = half < 0 ? COLS_PER_GROUP : COLS_PER_GROUP / 2;
             const int col_base = nb * BN + (half < 0 ? grp * COLS_PER_GROUP : half * (BN / 2) + grp * (COLS_PER_GROUP / 2));
             __nv_bfloat16* crow = p.C + ((int64_t)b * p.M + (row_ok ? row : 0)) * p.ldc;
+            const __nv_bfloat16* rrow = kEpi && p.residual && row_ok ? p.residual + ((int64_t)b * p.M + row) * p.N : nullptr;
+            if constexpr (kEpi) {       // the row's residuals go towards L2 while the tile is computed
+                if (rrow)
+                    for (int c = 0; c < cols && col_base + c < p.N; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(rrow + col_base + c));
+            }
 
             if constexpr (!kBlockScale) {
                 const float sa = row_ok ? __ldg(p.sa + (int64_t)b * p.M + row) : 0.0f;
@@ -554,8 +624,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 for (int c = 0; c < cols; c += 32) {
                     uint32_t r[32];
                     tmem_ld32(t_addr + c, r);
-                    tmem_ld_wait();
                     const int col0 = col_base + c;
+                    uint4 res[4];
+                    if constexpr (kEpi) load_residual<32>(rrow, col0, p.N, res);
+                    tmem_ld_wait();
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {          // N % 8 == 0: a group of 8 columns is all in or all out
@@ -570,6 +642,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[j + i] = __uint_as_float(r[j + i]) * sa * sv[i] + bv[i];
+                    }
+                    if constexpr (kEpi) {
+                        apply_act<32>(v, p.act);
+                        add_residual<32>(res, v);
                     }
                     if (row_ok) store_row32(crow, col0, p.N, v, wide);
                 }
@@ -602,6 +678,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     }
                     const float4* sa_s = sa_slots + (size_t)sbuf * (kScaleChunk / 4) * EPI_THREADS;
                     const float* sb_s = sb_slots + (size_t)sbuf * EPI_WARPS * kScaleChunk;
+                    const float* sbu_s = sbu_slots + (size_t)sbuf * EPI_WARPS * kScaleChunk;
                     const int kb_end = min(kbs - ch * kScaleChunk, kScaleChunk);
                     float4 sa4 = sa_s[0];
                 for (int kk = 0; kk < kb_end; ++kk) {
@@ -609,11 +686,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const float sa_k = sub == 0 ? sa4.x : sub == 1 ? sa4.y : sub == 2 ? sa4.z : sa4.w;
                     const float sc = sa_k * sb_s[kk];
                     const float2 s2 = make_float2(sc, sc);
+                    // gated: columns 0-63 of the accumulators are the thread's gate columns, 64-127 its up columns
+                    const float scu = kGated ? sa_k * sbu_s[kk] : sc;
+                    const float2 s2u = make_float2(scu, scu);
                     if (sub == 3 && kk + 1 < kb_end) sa4 = sa_s[(size_t)((kk + 1) >> 2) * EPI_THREADS];
                     if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar(acc), acc_ph, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
                     tc_fence_after();
                     if constexpr (kTrace) trace_at(12 + ew, ch * kScaleChunk + kk, lane == 0 && t == tile0 + 2 * tile_step, clock64());
-                    const uint32_t t_addr = tmem_base + lane_addr + acc * BN + grp * COLS_PER_GROUP;
+                    const uint32_t t_addr = tmem_base + lane_addr + acc * BN + grp * (kGated ? 64 : COLS_PER_GROUP);
+                    constexpr int kHalf2 = kGated ? BN / 2 : 64;           // where the second 64 columns start
                     uint32_t ra[32], rb[32];
                     // the partial product lives in registers after the fourth load: the TMEM buffer goes back
                     // to the MMA thread before the last FMAs
@@ -632,18 +713,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc2[j] = ffma2(ra[2 * j], ra[2 * j + 1], s2, acc2[j]);
                     tmem_ld_wait32(rb);
-                    tmem_ld32(t_addr + 64, ra);
+                    tmem_ld32(t_addr + kHalf2, ra);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc2[16 + j] = ffma2(rb[2 * j], rb[2 * j + 1], s2, acc2[16 + j]);
                     tmem_ld_wait32(ra);
-                    tmem_ld32(t_addr + 96, rb);
+                    tmem_ld32(t_addr + kHalf2 + 32, rb);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc2[32 + j] = ffma2(ra[2 * j], ra[2 * j + 1], s2, acc2[32 + j]);
+                    for (int j = 0; j < 16; ++j) acc2[32 + j] = ffma2(ra[2 * j], ra[2 * j + 1], s2u, acc2[32 + j]);
                     tmem_ld_wait32(rb);
                     release();
                     if constexpr (kTrace) trace_at(4 + ew, ch * kScaleChunk + kk, lane == 0 && t == tile0 + 2 * tile_step, clock64());
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc2[48 + j] = ffma2(rb[2 * j], rb[2 * j + 1], s2, acc2[48 + j]);
+                    for (int j = 0; j < 16; ++j) acc2[48 + j] = ffma2(rb[2 * j], rb[2 * j + 1], s2u, acc2[48 + j]);
                     if (++acc == 2) { acc = 0; acc_ph ^= 1; }
                 }
                     sbuf ^= 1;
@@ -676,6 +757,67 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                                 }
                             }
                             __syncwarp();
+                        }
+                    }
+                } else if constexpr (kGated) {
+                    if (ok) {
+                        float* const y = reinterpret_cast<float*>(acc2);
+#pragma unroll
+                        for (int j = 0; j < 64; j += 16) {
+                            apply_act<16>(y + j, p.act);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[j + i] *= y[64 + j + i];
+                        }
+                        const int F = p.N / 2, out0 = nb * (BN / 2) + grp * 64;
+                        if (BN == 256 && p.q_out) {
+                            float am = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) am = max_nan(am, fabsf(y[j]));
+                            // the other half of the row is the other warp's; the two tiles' worth of slots alternate: a warp is back
+                            // at a slot only after its partner has read it, since in between it waits for the partner's next maximum
+                            float* const slots = reinterpret_cast<float*>(smem + L::kStageOutOffset + kGatedSbBytes) + (max_n & 1) * 256;
+                            const uint32_t xb = max_bar((max_n & 1) * 4 + quarter);
+                            slots[ew * 32 + lane] = am;
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(xb);
+                            if (!__all_sync(0xFFFFFFFFu, mbar_wait(xb, (max_n >> 1) & 1, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
+                            am = max_nan(am, slots[(ew ^ 4) * 32 + lane]);
+                            ++max_n;
+                            const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f), rs = __frcp_rn(scale);
+                            if (row_ok) {
+                                uint32_t o[16];
+#pragma unroll
+                                for (int j = 0; j < 16; ++j)
+                                    o[j] = (uint32_t)cvt_e4m3x2(y[4 * j] * rs, y[4 * j + 1] * rs) | ((uint32_t)cvt_e4m3x2(y[4 * j + 2] * rs, y[4 * j + 3] * rs) << 16);
+                                uint8_t* const dst = p.q_out + (int64_t)row * F + out0;
+#pragma unroll
+                                for (int j = 0; j < 16; j += 8)
+                                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                                                 ::"l"(dst + 4 * j), "r"(o[j]), "r"(o[j + 1]), "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]), "r"(o[j + 5]),
+                                                   "r"(o[j + 6]), "r"(o[j + 7]) : "memory");
+                                if (grp == 0) p.q_scale[(int64_t)row * (F / 128) + nb] = scale;
+                            }
+                        } else if (row_ok) {
+#pragma unroll
+                            for (int j = 0; j < 64; j += 16) store_bf16x16(p.C + (int64_t)row * F + out0 + j, y + j);
+                        }
+                    }
+                } else if constexpr (kEpi) {
+                    if (ok && row_ok) {
+#pragma unroll
+                        for (int h = 0; h < 128; h += 64) {      // all residuals of 64 columns are in flight at once; 128 do not fit the registers
+                            uint4 res[8];
+                            load_residual<64>(rrow, col_base + h, p.N, res);
+#pragma unroll
+                            for (int c = 0; c < 64; c += 16) {
+                                float v[16];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) { v[2 * i] = acc2[(h + c) / 2 + i].x; v[2 * i + 1] = acc2[(h + c) / 2 + i].y; }
+                                if (p.bias) add_bias<16>(p.bias, col_base + h + c, p.N, v);
+                                apply_act<16>(v, p.act);
+                                add_residual<16>(res + c / 8, v);
+                                store_bf16x16(crow + col_base + h + c, v);
+                            }
                         }
                     }
                 } else if (ok && row_ok) {
@@ -735,7 +877,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     if (lane == 0) { if constexpr (kPair) mbar_arrive_cluster(tempty_bar(acc), 0); else mbar_arrive(tempty_bar(acc)); }
                     if (++acc == 2) { acc = 0; acc_ph ^= 1; }
                 }
-                if (ok && row_ok) {
+                if (kEpi && ok && row_ok) {
+#pragma unroll
+                    for (int c = 0; c < COLS_PER_GROUP; c += 32) {
+                        uint4 res[4];
+                        load_residual<32>(rrow, col_base + c, p.N, res);
+                        if (p.bias) add_bias<32>(p.bias, col_base + c, p.N, accv + c);
+                        apply_act<32>(accv + c, p.act);
+                        add_residual<32>(res, accv + c);
+                        store_row32(crow, col_base + c, p.N, accv + c, wide);
+                    }
+                } else if (ok && row_ok) {
 #pragma unroll
                     for (int c = 0; c < COLS_PER_GROUP; c += 32) {
                         if (p.c_a) mul_add_cols<32>(p.c_a, p.c_b, (int64_t)row * p.N + col_base + c, accv + c);
@@ -809,11 +961,11 @@ int launch_concat_cols(const void* src, void* dst, int64_t rows, int64_t w, int6
 
 namespace {
 // CTA-pair launch: clusters of 2 along x, one cluster per pair of SMs, persistent over 256 x 256 tiles.
-template <int STAGES, bool kBlockScale>
+template <int STAGES, bool kBlockScale, int kOut = 0>
 int launch_gemm_pair(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmBHalf, GemmParams p, cudaStream_t st) {
     using L = SmemLayout<256, STAGES, true, BM, kBlockScale ? 256 : 0>;
     static_assert(L::kDynamic <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
-    auto kern = gemm_fp8_kernel<256, STAGES, kBlockScale, true, true>;
+    auto kern = gemm_fp8_kernel<256, STAGES, kBlockScale, true, true, BM, kOut>;
     HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic));
     const int sms = sm_count();
     HKB_REQUIRE(sms > 1, HKB_ERR_CUDA, "no CUDA device");
@@ -828,7 +980,7 @@ int launch_gemm_pair(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
     p.split_from = tiles > clusters && 2 * last <= clusters ? tiles - last : tiles;
     const int threads = gemm_threads<256, kBlockScale, true>();
     HKB_CUDA(launch_dependent(starts_early(tiles, clusters), kern, 2 * clusters, threads, L::kDynamic, 2, st, tmA, tmB, p, tmBHalf));
-    note_kernel(kBlockScale ? "gemm_fp8_kernel<256,blockscale,pair>" : "gemm_fp8_kernel<256,pts,pair>");
+    note_kernel(kOut == 5 ? "gemm_fp8_kernel<256,pts,pair,epilogue>" : kBlockScale ? "gemm_fp8_kernel<256,blockscale,pair>" : "gemm_fp8_kernel<256,pts,pair>");
     return check_launch("gemm_fp8_kernel (CTA pairs)");
 }
 
@@ -851,8 +1003,7 @@ inline bool skinny_enabled() {
 
 template <int BN, int STAGES, bool kBlockScale, bool kGn128 = false, int AROWS = BM, int kOut = 0>
 int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p, cudaStream_t st) {
-    using L = SmemLayout<BN, STAGES, false, AROWS, (kBlockScale && kGn128) ? (BN == 256 ? 256 : 128) : 0, kOut == 1 ? 16 : 32,
-                         kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 : 0>;
+    using L = SmemLayout<BN, STAGES, false, AROWS, (kBlockScale && kGn128) ? (BN == 256 ? 256 : 128) : 0, kOut == 1 ? 16 : 32, stage_out_bytes<BN, kOut>()>;
     static_assert(L::kDynamic <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
     auto kern = gemm_fp8_kernel<BN, STAGES, kBlockScale, kGn128, false, AROWS, kOut>;
     // the attribute is per device; set it on every call (cheap) so multi-device processes work
@@ -866,6 +1017,9 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
                 kOut == 2 ? (kGn128 ? "gemm_fp8_kernel<128,blockscale,split_cat>" : "gemm_fp8_kernel<128,blockscale,gn1,split_cat>") :
                 kOut == 3 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,grouped>" : "gemm_fp8_kernel<128,blockscale,grouped>") :
                 kOut == 4 ? "gemm_fp8_kernel<256,blockscale,timeline>" :
+                kOut == 5 ? (kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,epilogue>" : kGn128 ? "gemm_fp8_kernel<128,blockscale,epilogue>" : "gemm_fp8_kernel<128,blockscale,gn1,epilogue>")
+                                         : (BN == 256 ? "gemm_fp8_kernel<256,pts,epilogue>" : BN == 128 ? "gemm_fp8_kernel<128,pts,epilogue>" : "gemm_fp8_kernel<64,pts,epilogue>")) :
+                kOut == 6 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,gated>" : "gemm_fp8_kernel<128,blockscale,gated>") :
                 kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale>" : kGn128 ? "gemm_fp8_kernel<128,blockscale>" : "gemm_fp8_kernel<128,blockscale,gn1>")
                             : (BN == 256 ? "gemm_fp8_kernel<256,pts>" : BN == 128 ? "gemm_fp8_kernel<128,pts>" : "gemm_fp8_kernel<64,pts>"));
     return check_launch("gemm_fp8_kernel");
@@ -884,36 +1038,24 @@ int common_checks(const char* who, const void* A, const void* B, const void* C, 
 
 }  // namespace
 
+struct Epilogue { const void* bias; int act; const void* residual; };
+int check_epilogue(const char* who, const Epilogue& ep) {
+    HKB_REQUIRE(act_known(ep.act), HKB_ERR_BAD_ARG, "%s: unknown activation %d", who, ep.act);
+    HKB_REQUIRE((!ep.bias || aligned16(ep.bias)) && (!ep.residual || aligned16(ep.residual)), HKB_ERR_BAD_ALIGN,
+                "%s: bias and residual must be 16-byte aligned", who);
+    return HKB_OK;
+}
 struct SplitCat { void* c2; int64_t s1, s2, s3; };      // C is c1 [M, D, s1+s3], c2 [M, D, s2], N = D*(s1+s2)
 int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float* sa, const float* sb, int64_t gn,
                              const void* c_a, const void* c_b, int64_t M, int64_t N, int64_t K, void* stream,
                              int64_t ldc = 0, void* const* peers = nullptr, int n_peer = 0, const SplitCat* sc = nullptr,
-                             unsigned long long* trace = nullptr);
+                             unsigned long long* trace = nullptr, const Epilogue* ep = nullptr);
 
-// wait_ns / skip_kblock: production passes kWaitLimitNs / -1; the wait-limit probe a short limit
-// and a K block that the producer leaves unloaded.
-int gemm_fp8_pts_impl(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias,
-                      int64_t batch, int64_t M, int64_t N, int64_t K, void* stream, uint64_t wait_ns, int skip_kblock) {
-    int rc = common_checks("gemm_fp8_pts", A, B, C, batch, M, N, K);
-    if (rc != HKB_OK) return rc;
-    HKB_REQUIRE(sa && sb, HKB_ERR_BAD_ARG, "gemm_fp8_pts: null scale pointer");
-    // the epilogues read b_scale four floats and the bias eight bf16 at a time
-    HKB_REQUIRE((reinterpret_cast<uintptr_t>(sa) & 3) == 0 && aligned16(sb) && (!bias || aligned16(bias)), HKB_ERR_BAD_ALIGN,
-                "gemm_fp8_pts: a_scale must be 4-byte, b_scale and bias 16-byte aligned");
-    GemmParams p{};
-    p.group_m = group_m_default();
-    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.batch = (int)batch;
-    p.sa = sa; p.sb = sb; p.bias = (const __nv_bfloat16*)bias; p.C = (__nv_bfloat16*)C; p.gn = 0;
-    p.ldc = N; p.n_peer = 0;
-    p.wait_ns = wait_ns; p.skip_kblock = skip_kblock;
-    rc = status_word(&p.status);
-    if (rc != HKB_OK) return rc;
-    // Decode shapes: HBM-bound on the weight stream; a kernel that deals the columns out evenly
-    // over the SMs (gemm_fp8_skinny.cu).  HKB_GEMM_SKINNY=0 keeps the fixed-width tiles below.
-    if (M <= 64 && batch == 1 && N % 16 == 0 && aligned32(C) && skip_kblock < 0 && skinny_enabled()) {
-        note_kernel("gemm_fp8_skinny_kernel");
-        return launch_gemm_fp8_skinny(A, B, C, sa, sb, bias, M, N, K, p.status, (cudaStream_t)stream);
-    }
+namespace {
+// Per-token tiles: `p` complete but for the tile counts.  kOut: 0 plain, 5 with activation and residual.
+template <int kOut>
+int launch_pts(const void* A, const void* B, GemmParams p, cudaStream_t st) {
+    const int64_t M = p.M, N = p.N, K = p.K, batch = p.batch;
     p.m_blks = (int)((M + BM - 1) / BM);
     // Skinny M: fetch only the rows that exist (rounded up to 8); the remaining rows of the
     // smem tile hold stale bytes that only reach accumulator rows >= M, which are never stored.
@@ -926,9 +1068,8 @@ int gemm_fp8_pts_impl(const void* A, const void* B, void* C, const float* sa, co
     if ((int64_t)p.m_blks * ((N + 255) / 256) * batch < 2LL * sms) bn = 128;
     if ((int64_t)p.m_blks * ((N + 127) / 128) * batch < 2LL * sms) bn = 64;
     p.n_blks = (int)((N + bn - 1) / bn);
-    cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap tmA, tmB;
-    rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, (uint64_t)batch, (uint32_t)p.a_box_rows);
+    int rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, (uint64_t)batch, (uint32_t)p.a_box_rows);
     if (rc != HKB_OK) return rc;
     // Large problems: CTA pairs on 256 x 256 tiles (a third less operand traffic per SM).
     const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256) * batch;
@@ -939,16 +1080,46 @@ int gemm_fp8_pts_impl(const void* A, const void* B, void* C, const float* sa, co
         CUtensorMap tmBHalf;
         rc = make_tmap_bytes(&tmBHalf, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, 64);
         if (rc != HKB_OK) return rc;
-        return launch_gemm_pair<7, false>(tmA, tmB, tmBHalf, p, st);
+        return launch_gemm_pair<7, false, kOut>(tmA, tmB, tmBHalf, p, st);
     }
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, (uint32_t)bn);
     if (rc != HKB_OK) return rc;
-    if (bn == 256) return launch_gemm<256, 4, false>(tmA, tmB, p, st);
-    if (bn == 128) return launch_gemm<128, 6, false>(tmA, tmB, p, st);
+    if (bn == 256) return launch_gemm<256, 4, false, false, BM, kOut>(tmA, tmB, p, st);
+    if (bn == 128) return launch_gemm<128, 6, false, false, BM, kOut>(tmA, tmB, p, st);
     // skinny M with narrow tiles (decode shapes): stage only the A rows that exist, deepen the ring
-    if (p.a_box_rows <= 16) return launch_gemm<64, 19, false, false, 16>(tmA, tmB, p, st);
-    if (p.a_box_rows <= 64) return launch_gemm<64, 12, false, false, 64>(tmA, tmB, p, st);
-    return launch_gemm<64, 8, false>(tmA, tmB, p, st);
+    if (p.a_box_rows <= 16) return launch_gemm<64, 19, false, false, 16, kOut>(tmA, tmB, p, st);
+    if (p.a_box_rows <= 64) return launch_gemm<64, 12, false, false, 64, kOut>(tmA, tmB, p, st);
+    return launch_gemm<64, 8, false, false, BM, kOut>(tmA, tmB, p, st);
+}
+}  // namespace
+
+// wait_ns / skip_kblock: production passes kWaitLimitNs / -1; the wait-limit probe a short limit
+// and a K block that the producer leaves unloaded.
+int gemm_fp8_pts_impl(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias,
+                      int64_t batch, int64_t M, int64_t N, int64_t K, void* stream, uint64_t wait_ns, int skip_kblock, const Epilogue* ep = nullptr) {
+    int rc = common_checks("gemm_fp8_pts", A, B, C, batch, M, N, K);
+    if (rc != HKB_OK) return rc;
+    HKB_REQUIRE(sa && sb, HKB_ERR_BAD_ARG, "gemm_fp8_pts: null scale pointer");
+    // the epilogues read b_scale four floats and the bias eight bf16 at a time
+    HKB_REQUIRE((reinterpret_cast<uintptr_t>(sa) & 3) == 0 && aligned16(sb) && (!bias || aligned16(bias)), HKB_ERR_BAD_ALIGN,
+                "gemm_fp8_pts: a_scale must be 4-byte, b_scale and bias 16-byte aligned");
+    GemmParams p{};
+    p.group_m = group_m_default();
+    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.batch = (int)batch;
+    p.sa = sa; p.sb = sb; p.bias = (const __nv_bfloat16*)bias; p.C = (__nv_bfloat16*)C; p.gn = 0;
+    p.ldc = N; p.n_peer = 0;
+    if (ep) { p.act = ep->act; p.residual = (const __nv_bfloat16*)ep->residual; }
+    p.wait_ns = wait_ns; p.skip_kblock = skip_kblock;
+    rc = status_word(&p.status);
+    if (rc != HKB_OK) return rc;
+    // Decode shapes: HBM-bound on the weight stream; a kernel that deals the columns out evenly
+    // over the SMs (gemm_fp8_skinny.cu).  HKB_GEMM_SKINNY=0 keeps the fixed-width tiles below.
+    if (M <= 64 && batch == 1 && N % 16 == 0 && aligned32(C) && skip_kblock < 0 && skinny_enabled()) {
+        note_kernel(ep ? "gemm_fp8_skinny_kernel<epilogue>" : "gemm_fp8_skinny_kernel");
+        return launch_gemm_fp8_skinny(A, B, C, sa, sb, bias, ep ? &ep->act : nullptr, ep ? ep->residual : nullptr, M, N, K, p.status, (cudaStream_t)stream);
+    }
+    if (ep) return launch_pts<5>(A, B, p, (cudaStream_t)stream);
+    return launch_pts<0>(A, B, p, (cudaStream_t)stream);
 }
 }  // namespace hkb
 
@@ -957,6 +1128,24 @@ extern "C" {
 int hkb_gemm_fp8_pts(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias,
                      int64_t batch, int64_t M, int64_t N, int64_t K, void* stream) {
     return hkb::gemm_fp8_pts_impl(A, B, C, sa, sb, bias, batch, M, N, K, stream, hkb::kWaitLimitNs, -1);
+}
+
+int hkb_gemm_fp8_pts_epilogue(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias, int act,
+                              const void* residual, int64_t batch, int64_t M, int64_t N, int64_t K, void* stream) {
+    using namespace hkb;
+    const Epilogue ep{bias, act, residual};
+    const int rc = check_epilogue("gemm_fp8_pts_epilogue", ep);
+    if (rc != HKB_OK) return rc;
+    return gemm_fp8_pts_impl(A, B, C, sa, sb, bias, batch, M, N, K, stream, kWaitLimitNs, -1, &ep);
+}
+
+int hkb_gemm_fp8_blockscale_epilogue(const void* A, const void* B, void* C, const float* sa, const float* sb, int64_t gn, const void* bias,
+                                     int act, const void* residual, int64_t M, int64_t N, int64_t K, void* stream) {
+    using namespace hkb;
+    const Epilogue ep{bias, act, residual};
+    const int rc = check_epilogue("gemm_fp8_blockscale_epilogue", ep);
+    if (rc != HKB_OK) return rc;
+    return gemm_fp8_blockscale_impl(A, B, C, sa, sb, gn, nullptr, nullptr, M, N, K, stream, 0, nullptr, 0, nullptr, nullptr, &ep);
 }
 
 int hkb_debug_gemm_fp8_wait_probe(const void* A, const void* B, void* C, const float* sa, const float* sb,
@@ -1072,7 +1261,7 @@ namespace hkb {
 
 int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float* sa, const float* sb, int64_t gn,
                              const void* c_a, const void* c_b, int64_t M, int64_t N, int64_t K, void* stream,
-                             int64_t ldc, void* const* peers, int n_peer, const SplitCat* sc, unsigned long long* trace) {
+                             int64_t ldc, void* const* peers, int n_peer, const SplitCat* sc, unsigned long long* trace, const Epilogue* ep) {
     int rc = common_checks("gemm_fp8_blockscale", A, B, C, 1, M, N, K);
     if (rc != HKB_OK) return rc;
     if (sc) {
@@ -1099,6 +1288,7 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     p.sa = sa; p.sb = sb; p.bias = nullptr; p.C = (__nv_bfloat16*)C; p.gn = (int)gn;
     p.c_a = (const __nv_bfloat16*)c_a; p.c_b = (const __nv_bfloat16*)c_b;
     p.ldc = ldc; p.n_peer = n_peer;
+    if (ep) { p.bias = (const __nv_bfloat16*)ep->bias; p.act = ep->act; p.residual = (const __nv_bfloat16*)ep->residual; }
     for (int d = 0; d < n_peer; ++d) p.peer[d] = (__nv_bfloat16*)peers[d];
     if (sc) { p.c2 = (__nv_bfloat16*)sc->c2; p.sc_s1 = (int)sc->s1; p.sc_s2 = (int)sc->s2; p.sc_s3 = (int)sc->s3; }
     p.wait_ns = kWaitLimitNs; p.skip_kblock = -1;
@@ -1107,8 +1297,12 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     // Decode shapes: the weight stream bounds them (gemm_fp8_blockscale_skinny.cu).  At 32 tokens it is
     // ahead for every N and K tried, at 64 behind (figures there).
     if (M <= 32 && gn == 128 && !sc && n_peer == 0 && !trace) {
-        note_kernel("gemm_fp8_blockscale_skinny_kernel");
-        return launch_gemm_fp8_blockscale_skinny(A, B, C, sa, sb, c_a, c_b, M, N, K, ldc, p.status, (cudaStream_t)stream);
+        note_kernel(ep ? "gemm_fp8_blockscale_skinny_kernel<epilogue>" : "gemm_fp8_blockscale_skinny_kernel");
+        BsSkinnyOut out{C, ldc};
+        out.c_a = c_a;
+        out.c_b = c_b;
+        if (ep) { out.epilogue = true; out.bias = ep->bias; out.act = ep->act; out.residual = ep->residual; }
+        return launch_gemm_fp8_blockscale_skinny(A, B, sa, sb, out, M, N, K, p.status, (cudaStream_t)stream);
     }
     p.m_blks = (int)((M + BM - 1) / BM);
     p.a_box_rows = BM;
@@ -1133,7 +1327,7 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     // reachable for experiments only.
     static const bool bs_pairs = [] { const char* v = getenv("HKB_BLOCKSCALE_PAIRS"); return v && v[0] == '1'; }();
     const int64_t pair_tiles = ((M + 255) / 256) * (N / 256);
-    if (bs_pairs && bn == 256 && M > 128 && pair_tiles >= sms / 2) {
+    if (bs_pairs && !ep && bn == 256 && M > 128 && pair_tiles >= sms / 2) {
         p.m_blks = (int)((M + 255) / 256);
         rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)N, 1, 128);
         if (rc != HKB_OK) return rc;
@@ -1149,6 +1343,11 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
         if (bn == 256) return launch_gemm<256, 3, true, true, BM, 1>(tmA, tmB, p, st);
         return launch_gemm<128, 5, true, true, BM, 1>(tmA, tmB, p, st);
     }
+    if (ep) {
+        if (gn != 128) return launch_gemm<128, 6, true, false, BM, 5>(tmA, tmB, p, st);
+        if (bn == 256) return launch_gemm<256, 3, true, true, BM, 5>(tmA, tmB, p, st);
+        return launch_gemm<128, 5, true, true, BM, 5>(tmA, tmB, p, st);
+    }
     if (gn == 128) {
         if (bn == 256) return launch_gemm<256, 3, true, true>(tmA, tmB, p, st);
         return launch_gemm<128, 5, true, true>(tmA, tmB, p, st);
@@ -1156,4 +1355,72 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     return launch_gemm<128, 6, true, false>(tmA, tmB, p, st);
 }
 
+namespace {
+// Gated GEMM.  Up to 32 tokens the decode kernel deals the output columns out in tiles that do not keep to 128-column scale groups:
+// its FP8 output goes through fp32 in the caller's workspace and a second, small launch.
+constexpr int64_t kGatedDecodeRows = 32;
+int check_gated(int64_t M, int64_t F, int64_t K) {
+    HKB_REQUIRE(M >= 1 && F >= 1 && K >= 1 && F % 128 == 0 && K % 128 == 0, HKB_ERR_BAD_SHAPE,
+                "gemm_fp8_blockscale_gated: need M > 0 and F and K positive multiples of 128, got M=%lld F=%lld K=%lld", (long long)M, (long long)F, (long long)K);
+    HKB_REQUIRE(M < (1LL << 31) && F < (1LL << 30) && K < (1LL << 31), HKB_ERR_BAD_SHAPE, "gemm_fp8_blockscale_gated: dimension too large");
+    return HKB_OK;
+}
+}  // namespace
 }  // namespace hkb
+
+extern "C" {
+
+int64_t hkb_gemm_fp8_blockscale_gated_workspace(int64_t M, int64_t F, int64_t K, int fp8_output) {
+    using namespace hkb;
+    const int rc = check_gated(M, F, K);
+    if (rc != HKB_OK) return rc;
+    return fp8_output && M <= kGatedDecodeRows ? M * F * 4 : 0;
+}
+
+int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* c_scale, const float* sa, const float* sb, int act,
+                                  void* workspace, int64_t M, int64_t F, int64_t K, void* stream) {
+    using namespace hkb;
+    HKB_REQUIRE(A && B && C && sa && sb, HKB_ERR_BAD_ARG, "gemm_fp8_blockscale_gated: null pointer");
+    HKB_REQUIRE(act_known(act), HKB_ERR_BAD_ARG, "gemm_fp8_blockscale_gated: unknown activation %d", act);
+    int rc = check_gated(M, F, K);
+    if (rc != HKB_OK) return rc;
+    HKB_REQUIRE(aligned16(A) && aligned16(B) && aligned32(C) && ((uintptr_t)c_scale & 3) == 0 && ((uintptr_t)sa & 3) == 0 && ((uintptr_t)sb & 3) == 0,
+                HKB_ERR_BAD_ALIGN, "gemm_fp8_blockscale_gated: A and B must be 16-byte, C 32-byte, scales 4-byte aligned");
+    HKB_REQUIRE(hkb_gemm_fp8_blockscale_gated_workspace(M, F, K, c_scale != nullptr) == 0 || (workspace && aligned16(workspace)), HKB_ERR_BAD_ARG,
+                "gemm_fp8_blockscale_gated: this size needs a 16-byte aligned workspace");
+    cudaStream_t st = (cudaStream_t)stream;
+    uint32_t* status = nullptr;
+    rc = status_word(&status);
+    if (rc != HKB_OK) return rc;
+    if (M <= kGatedDecodeRows) {
+        note_kernel("gemm_fp8_blockscale_skinny_kernel<gated>");
+        BsSkinnyOut out{C, F};
+        out.gated = true;
+        out.act = act;
+        out.f32 = c_scale ? (float*)workspace : nullptr;
+        rc = launch_gemm_fp8_blockscale_skinny(A, B, sa, sb, out, M, F, K, status, st);
+        if (rc != HKB_OK || !c_scale) return rc;
+        return launch_quant_f32_1x128((const float*)workspace, C, c_scale, M * (F / 128), st);
+    }
+    GemmParams p{};
+    p.group_m = group_m_env() ? group_m_env() : 16;
+    p.M = (int)M; p.N = (int)(2 * F); p.K = (int)K; p.batch = 1;
+    p.sa = sa; p.sb = sb; p.gn = 128; p.ldc = F; p.act = act;
+    if (c_scale) { p.q_out = (uint8_t*)C; p.q_scale = c_scale; } else p.C = (__nv_bfloat16*)C;
+    p.wait_ns = kWaitLimitNs; p.skip_kblock = -1; p.status = status;
+    p.m_blks = (int)((M + BM - 1) / BM);
+    p.a_box_rows = BM;
+    // 128 output columns per tile where that gives every SM two tiles, as in the plain GEMM, and for FP8 output always: a tile has
+    // to hold whole scale groups
+    const int bn = c_scale || p.m_blks * (F / 128) >= 2LL * sm_count() ? 256 : 128;
+    p.n_blks = (int)(F / (bn / 2));
+    CUtensorMap tmA, tmB;
+    rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, 1, BM);
+    if (rc != HKB_OK) return rc;
+    rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)(2 * F), 1, (uint32_t)bn / 2);
+    if (rc != HKB_OK) return rc;
+    if (bn == 256) return launch_gemm<256, 3, true, true, BM, 6>(tmA, tmB, p, st);
+    return launch_gemm<128, 5, true, true, BM, 6>(tmA, tmB, p, st);
+}
+
+}  // extern "C"

@@ -24,8 +24,12 @@
 // 17 x 28672 x 8192 78.9 / 62.5 (c_a and c_b loaded token by token behind the stores instead: 21.5, 27.7, 76.8).  With 64
 // tokens the epilogue's scale reads take over (64 x 28672 x 8192 57.4 / 64.6): those stay there.
 //
+// Gated (kOut == 2): a tile is up to 64 output columns, its MMA rows the gate rows of those columns and behind them the up rows (two
+// boxes).  Behind the last K block the threads of the up rows hand their sums to those of the gate rows through shared memory.
+//
 // Roles: warp 0 TMA producer, warp 1 TMEM allocator + MMA issuer, warps 2-9 epilogue, warps 10-11 scale staging.  Bounded
 // waits and teardown as in gemm_fp8.cu.
+#include "activation.cuh"
 #include "tc_common.cuh"
 
 namespace hkb {
@@ -36,9 +40,12 @@ constexpr int kStep = 2;                  // K blocks per pipeline stage, hand-o
 constexpr int kAccs = 8;                  // accumulator sets in TMEM, kStep partial products of 32 columns each
 constexpr int kSlots = 4;                 // ring of staged scales
 constexpr int kChunk = 8;                 // K blocks per slot
-constexpr int kPitch = 36;                // floats per K block: 32 token scales, then the weight scales of two groups
+constexpr int kPitch = 36;                // floats per K block: 32 token scales, then the weight scales of two groups (gated: two of gate, two of up)
 constexpr int kSlotBytes = kChunk * kPitch * 4;
 constexpr int kHeadBytes = 1024 * ((1024 + kSlots * kSlotBytes + 1023) / 1024);      // barriers (first KB), then the scale ring
+constexpr int kXchgPitch = 65;            // gated: up sums [token][64 rows], one float of padding
+constexpr int kXchgBytes = 9 * 1024;
+static_assert(32 * kXchgPitch * 4 <= kXchgBytes, "exchange area");
 constexpr int kTailPad = 16 * 1024;       // the MMA reads 128 weight rows from every stage base
 constexpr int kSmemLimit = 232448;        // 227 KB
 constexpr int kMaxUnits = 8;              // 128 weight rows
@@ -56,6 +63,10 @@ struct BsSkinnyParams {
     __nv_bfloat16* C;
     const __nv_bfloat16* c_a;             // fused multiply-add (both [M, N]), or null
     const __nv_bfloat16* c_b;
+    const __nv_bfloat16* bias;            // kOut == 1: act(gemm + bias[n]) + residual[m, n], either null
+    const __nv_bfloat16* residual;
+    int act;                              // kOut == 1, 2
+    float* f32;                           // kOut == 2: the result [M, N] in fp32 instead of C, or null
     uint32_t* status;
 };
 
@@ -67,22 +78,25 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
 #define TILE_UNITS(t) (p.base + ((t) < p.rem ? 1 : 0))
 #define TILE_ROW0(t) (((t) * p.base + min((t), p.rem)) * 16)
 
-// NT: token columns (16 or 32).
-template <int NT>
+// NT: token columns (16 or 32).  kOut: 0 plain / multiply-add, 1 bias + activation + residual, 2 gated (p.N output columns, B has 2N rows).
+template <int NT, int kOut>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                                   const __grid_constant__ CUtensorMap tmB1, const BsSkinnyParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t bar_base = smem_u32(smem);
-    const uint32_t ring_base = bar_base + kHeadBytes;
+    const uint32_t ring_base = bar_base + kHeadBytes + (kOut == 2 ? kXchgBytes : 0);
+    float* const xchg = reinterpret_cast<float*>(smem + kHeadBytes);
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kMaxStages + s); };
     auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * kMaxStages + a); };
     auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kMaxStages + kAccs + a); };
     auto sfull_bar = [&](int i) { return bar_base + 8u * (2 * kMaxStages + 2 * kAccs + i); };
     auto sempty_bar = [&](int i) { return bar_base + 8u * (2 * kMaxStages + 2 * kAccs + kSlots + i); };
-    constexpr int kNumBars = 2 * kMaxStages + 2 * kAccs + 2 * kSlots;
+    auto xfull_bar = [&](int i) { return bar_base + 8u * (2 * kMaxStages + 2 * kAccs + 2 * kSlots + i); };       // gated: 0 written, 1 read
+    constexpr bool kGated = kOut == 2;
+    constexpr int kNumBars = 2 * kMaxStages + 2 * kAccs + 2 * kSlots + 2;
     static_assert(kNumBars * 8 + 8 <= 1024, "barrier area");
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kNumBars * 8);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -109,6 +123,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
             mbar_init(sfull_bar(i), 1);
             mbar_init(sempty_bar(i), kEpiWarps);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(xfull_bar(i), kEpiWarps);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -130,7 +145,8 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
             for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
                 const CUtensorMap* const tmB = t < p.rem ? &tmB1 : &tmB0;
                 const int n0 = TILE_ROW0(t);
-                const uint32_t stage_tx = kStep * ((uint32_t)p.a_box_rows * 128 + (uint32_t)TILE_UNITS(t) * 2048);
+                const uint32_t b_bytes = (uint32_t)TILE_UNITS(t) * 2048;
+                const uint32_t stage_tx = kStep * ((uint32_t)p.a_box_rows * 128 + (kGated ? 2 : 1) * b_bytes);
                 for (int ks = 0; ks < ksteps; ++ks) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1, abort_flag, p.status, kErrWaitProducer)) { ok = false; break; }
                     mbar_arrive_expect_tx(full_bar(s), stage_tx);
@@ -138,6 +154,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
 #pragma unroll
                     for (int i = 0; i < kStep; ++i) {
                         tma_load_3d(st + i * p.sub_bytes, tmB, full_bar(s), (ks * kStep + i) * 128, n0, 0);
+                        if constexpr (kGated) tma_load_3d(st + i * p.sub_bytes + b_bytes, tmB, full_bar(s), (ks * kStep + i) * 128, p.N + n0, 0);
                         tma_load_3d(st + i * p.sub_bytes + p.a_off, &tmA, full_bar(s), (ks * kStep + i) * 128, 0, 0);
                     }
                     if (++s == p.stages) { s = 0; ph ^= 1; }
@@ -180,16 +197,22 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         int acc = 0, slot = 0, s = 0;
-        uint32_t acc_ph = 0, slot_ph = 0;
+        uint32_t acc_ph = 0, slot_ph = 0, x_ph = 0;
         bool ok = true;
         for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
-            const int rows = TILE_UNITS(t) * 16;
+            const int cols = TILE_UNITS(t) * 16;                         // output columns of the tile
+            const int rows = kGated ? 2 * cols : cols;
             const int n0 = TILE_ROW0(t);
             const bool row_ok = row_in_tile < rows;
             const bool warp_has_rows = quarter * 32 < rows;              // warp-uniform
-            const int n = n0 + (row_ok ? row_in_tile : 0);
-            const int group = (n >> 7) - (n0 >> 7);                      // 0 or 1
-            if (p.c_a && warp_has_rows && col0 + (lane & (NC - 1)) < p.M) {      // this warp's part of c_a and c_b, into L2
+            const bool is_up = kGated && row_in_tile >= cols;
+            const int n = n0 + (row_ok ? row_in_tile - (is_up ? cols : 0) : 0);
+            const int group = (n >> 7) - (n0 >> 7) + (is_up ? 2 : 0);    // 0 or 1; gated: 2 or 3 for the up rows
+            if constexpr (kOut == 1) {
+                if (p.residual && warp_has_rows && lane < NC && col0 + lane < p.M)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + (int64_t)(col0 + lane) * p.N + n0 + quarter * 32));
+            }
+            if (kOut == 0 && p.c_a && warp_has_rows && col0 + (lane & (NC - 1)) < p.M) {      // this warp's part of c_a and c_b, into L2
                 const int64_t off = (int64_t)(col0 + (lane & (NC - 1))) * p.N + n0 + quarter * 32;
                 asm volatile("prefetch.global.L2 [%0];" ::"l"((lane < 16 ? p.c_a : p.c_b) + off));
             }
@@ -246,11 +269,52 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
                 if (lane == 0) mbar_arrive(sempty_bar(slot));
                 if (++slot == kSlots) { slot = 0; slot_ph ^= 1; }
             }
-            if (ok && row_ok) {
+            if constexpr (kGated) {
+                // the up sums change hands: written, all eight warps arrive, read by the gate rows, all arrive before the next tile writes
+                float* const xr = xchg + col0 * kXchgPitch + (n - n0);
+                if (ok && !__all_sync(0xFFFFFFFFu, mbar_wait(xfull_bar(1), x_ph ^ 1, abort_flag, p.status, kErrWaitEpilogue))) ok = false;
+                if (!ok) break;
+                if (row_ok && is_up) {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) xr[j * kXchgPitch] = (j & 1) ? acc2[j / 2].y : acc2[j / 2].x;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(xfull_bar(0));
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(xfull_bar(0), x_ph, abort_flag, p.status, kErrWaitEpilogue))) { ok = false; break; }
+                float v[NC], up[NC];
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    v[j] = (j & 1) ? acc2[j / 2].y : acc2[j / 2].x;
+                    up[j] = row_ok && !is_up ? xr[j * kXchgPitch] : 0.0f;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(xfull_bar(1));
+                x_ph ^= 1;
+                if (row_ok && !is_up) {
+                    apply_act<NC>(v, p.act);
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) {
+                        if (col0 + j >= p.M) break;
+                        if (p.f32) p.f32[(int64_t)(col0 + j) * p.N + n] = v[j] * up[j];
+                        else p.C[(int64_t)(col0 + j) * p.ldc + n] = __float2bfloat16_rn(v[j] * up[j]);
+                    }
+                }
+            } else if (ok && row_ok) {
                 float v[NC];
 #pragma unroll
                 for (int j = 0; j < NC; ++j) v[j] = (j & 1) ? acc2[j / 2].y : acc2[j / 2].x;
-                if (p.c_a) {
+                if constexpr (kOut == 1) {
+                    float res[NC];                  // loaded together and ahead of the stores, for the same reason
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) res[j] = p.residual ? __bfloat162float(p.residual[(int64_t)min(col0 + j, p.M - 1) * p.N + n]) : 0.0f;
+                    const float bn = p.bias ? __bfloat162float(p.bias[n]) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) v[j] += bn;
+                    apply_act<NC>(v, p.act);
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) v[j] += res[j];
+                }
+                if (kOut == 0 && p.c_a) {
                     // All loads go out before the first store: C may be c_a or c_b, so the compiler cannot move them up, and one
                     // round trip per token is longer than the whole K loop of a small layer.
                     __nv_bfloat16 ca[NC], cb[NC];
@@ -271,7 +335,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
     } else {
         // ================= scale staging: warp g fills every second slot =================
         const int g = warp - 2 - kEpiWarps;
-        const int nsb = p.N / 128;
+        const int nsb = p.N / 128;                           // gated: of gate and of up
         const bool vec = (kblocks & 3) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
         int slot = g, ch = g;                                // ch: chunk of the tile, in the epilogue's order
         uint32_t ph = 0;
@@ -293,13 +357,15 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
                         for (int i = 0; i < 4; ++i) v[k + i] = (lane < p.M && k + i < kn) ? __ldg(src + k + i) : 0.0f;
                     }
                 }
-                const int wk = lane >> 1, wg = min(g0 + (lane & 1), nsb - 1);
-                const float wsc = wk < kn ? __ldg(p.sb + (int64_t)(kb0 + wk) * nsb + wg) : 0.0f;
+                // two weight scales per K block (gated: two of gate, two of up)
+                constexpr int W = kGated ? 4 : 2;
+                const int wk = lane / W, wi = lane % W, wg = min(g0 + (wi & 1), nsb - 1) + (wi >> 1) * nsb;
+                const float wsc = wk < kn ? __ldg(p.sb + (int64_t)(kb0 + wk) * (W / 2 * nsb) + wg) : 0.0f;
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(sempty_bar(slot), ph ^ 1, abort_flag, p.status, kErrWaitProducer))) { ok = false; break; }
                 float* const dst = scales + slot * kChunk * kPitch;
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) dst[k * kPitch + lane] = v[k];
-                if (wk < kChunk) dst[wk * kPitch + 32 + (lane & 1)] = wsc;
+                if (wk < kChunk) dst[wk * kPitch + 32 + wi] = wsc;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sfull_bar(slot));
                 slot += 2;
@@ -324,48 +390,61 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
 #undef TILE_UNITS
 #undef TILE_ROW0
 
-template <int NT>
+template <int NT, int kOut>
 int launch(const CUtensorMap& tmA, const CUtensorMap& tmB0, const CUtensorMap& tmB1, const BsSkinnyParams& p, int smem, int grid, cudaStream_t st) {
     // the limit is the kernel's, not the call's: every call sets the same one, whatever its own size (calls may overlap)
-    HKB_CUDA(cudaFuncSetAttribute(gemm_fp8_blockscale_skinny_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
-    HKB_CUDA(launch_dependent(true, gemm_fp8_blockscale_skinny_kernel<NT>, grid, kThreads, smem, 0, st, tmA, tmB0, tmB1, p));
+    auto kern = gemm_fp8_blockscale_skinny_kernel<NT, kOut>;
+    HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    HKB_CUDA(launch_dependent(true, kern, grid, kThreads, smem, 0, st, tmA, tmB0, tmB1, p));
     return check_launch("gemm_fp8_blockscale_skinny_kernel");
+}
+
+template <int NT>
+int launch_out(const CUtensorMap& tmA, const CUtensorMap& tmB0, const CUtensorMap& tmB1, const BsSkinnyParams& p, const BsSkinnyOut& out, int smem,
+               int grid, cudaStream_t st) {
+    if (out.gated) return launch<NT, 2>(tmA, tmB0, tmB1, p, smem, grid, st);
+    if (out.epilogue) return launch<NT, 1>(tmA, tmB0, tmB1, p, smem, grid, st);
+    return launch<NT, 0>(tmA, tmB0, tmB1, p, smem, grid, st);
 }
 
 }  // namespace
 
-// Host side: called by gemm_fp8_blockscale_impl for M <= 32 and 128-column weight-scale groups (arguments already validated).
-int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* c_a, const void* c_b,
-                                      int64_t M, int64_t N, int64_t K, int64_t ldc, uint32_t* status, cudaStream_t st) {
+// Host side: called for M <= 32 and 128-column weight-scale groups (arguments already validated).
+int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, const float* sa, const float* sb, const BsSkinnyOut& out, int64_t M,
+                                      int64_t N, int64_t K, uint32_t* status, cudaStream_t st) {
     const int sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
     BsSkinnyParams p{};
-    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.ldc = ldc;
-    p.sa = sa; p.sb = sb; p.C = (__nv_bfloat16*)C; p.c_a = (const __nv_bfloat16*)c_a; p.c_b = (const __nv_bfloat16*)c_b; p.status = status;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.ldc = out.ldc;
+    p.sa = sa; p.sb = sb; p.C = (__nv_bfloat16*)out.C; p.c_a = (const __nv_bfloat16*)out.c_a; p.c_b = (const __nv_bfloat16*)out.c_b; p.status = status;
+    p.bias = (const __nv_bfloat16*)out.bias; p.act = out.act; p.residual = (const __nv_bfloat16*)out.residual; p.f32 = out.f32;
     p.a_box_rows = (int)((M + 7) / 8 * 8);
     const int nt = (int)((M + 15) / 16 * 16);
     const int64_t units = N / 16;
-    const int64_t rounds = (units + (int64_t)kMaxUnits * sms - 1) / ((int64_t)kMaxUnits * sms);
+    const int parts = out.gated ? 2 : 1;                  // gate and up rows share the 128 MMA rows
+    const int max_units = kMaxUnits / parts;
+    const int64_t rounds = (units + (int64_t)max_units * sms - 1) / ((int64_t)max_units * sms);
     p.tiles = (int)(units < rounds * sms ? units : rounds * sms);
     p.base = (int)(units / p.tiles);
     p.rem = (int)(units % p.tiles);
     const int maxu = p.base + (p.rem ? 1 : 0);
-    HKB_REQUIRE(maxu >= 1 && maxu <= kMaxUnits, HKB_ERR_UNSUPPORTED, "gemm_fp8_blockscale (skinny): internal tile height %d out of range", maxu);
-    p.a_off = maxu * 2048;
+    HKB_REQUIRE(maxu >= 1 && maxu <= max_units, HKB_ERR_UNSUPPORTED, "gemm_fp8_blockscale (skinny): internal tile height %d out of range", maxu);
+    p.a_off = parts * maxu * 2048;
     p.sub_bytes = p.a_off + nt * 128;
-    p.stages = (kSmemLimit - 1024 - kHeadBytes - kTailPad) / (kStep * p.sub_bytes);
+    const int head = kHeadBytes + (out.gated ? kXchgBytes : 0);
+    p.stages = (kSmemLimit - 1024 - head - kTailPad) / (kStep * p.sub_bytes);
     if (p.stages > kMaxStages) p.stages = kMaxStages;
-    const int smem = 1024 + kHeadBytes + p.stages * kStep * p.sub_bytes + kTailPad;
+    const int smem = 1024 + head + p.stages * kStep * p.sub_bytes + kTailPad;
     CUtensorMap tmA, tmB0, tmB1;
     int rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, 1, (uint32_t)p.a_box_rows);
     if (rc != HKB_OK) return rc;
-    rc = make_tmap_bytes(&tmB0, B, (uint64_t)K, (uint64_t)N, 1, (uint32_t)p.base * 16);
+    rc = make_tmap_bytes(&tmB0, B, (uint64_t)K, (uint64_t)(parts * N), 1, (uint32_t)p.base * 16);
     if (rc != HKB_OK) return rc;
-    rc = make_tmap_bytes(&tmB1, B, (uint64_t)K, (uint64_t)N, 1, (uint32_t)maxu * 16);
+    rc = make_tmap_bytes(&tmB1, B, (uint64_t)K, (uint64_t)(parts * N), 1, (uint32_t)maxu * 16);
     if (rc != HKB_OK) return rc;
     const int grid = p.tiles < sms ? p.tiles : sms;
-    if (nt == 16) return launch<16>(tmA, tmB0, tmB1, p, smem, grid, st);
-    return launch<32>(tmA, tmB0, tmB1, p, smem, grid, st);
+    if (nt == 16) return launch_out<16>(tmA, tmB0, tmB1, p, out, smem, grid, st);
+    return launch_out<32>(tmA, tmB0, tmB1, p, out, smem, grid, st);
 }
 
 }  // namespace hkb

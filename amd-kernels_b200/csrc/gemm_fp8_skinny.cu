@@ -28,6 +28,7 @@
 //
 // Roles, bounded waits and teardown as in gemm_fp8.cu: warp 0 TMA producer, warp 1 TMEM
 // allocator + MMA issuer, warps 2-5 epilogue (two TMEM accumulators of 256 columns).
+#include "activation.cuh"
 #include "tc_common.cuh"
 
 namespace hkb {
@@ -48,6 +49,8 @@ struct SkinnyParams {
     const float* sa;
     const float* sb;
     const __nv_bfloat16* bias;
+    const __nv_bfloat16* residual;      // kEpi: C = act(gemm + bias) + residual ([M, N] or null)
+    int act;
     __nv_bfloat16* C;
     uint32_t* status;
 };
@@ -63,6 +66,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 #define TILE_WIDTH(t) (p.base + ((t) < p.rem ? 1 : 0))
 #define TILE_COL0(t) (((t) * p.base + min((t), p.rem)) * 16)
 
+// kEpi: activation and residual behind the bias.
+template <bool kEpi>
 __global__ void __launch_bounds__(192, 1)
 gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                        const __grid_constant__ CUtensorMap tmB1,
@@ -181,8 +186,15 @@ gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 for (int u = 0; u < w; ++u) {
                     uint32_t r[16];
                     tmem_ld16(t_addr + u * 16, r);
-                    tmem_ld_wait();
                     const int col0 = n0 + u * 16;
+                    uint4 res[2];
+                    if constexpr (kEpi) {       // plain loads ahead of the stores: C may be the residual
+                        const uint4* const src = reinterpret_cast<const uint4*>(p.residual + (int64_t)row * p.N + col0);
+                        const bool has = p.residual && row_ok;
+                        res[0] = has ? src[0] : make_uint4(0, 0, 0, 0);
+                        res[1] = has ? src[1] : make_uint4(0, 0, 0, 0);
+                    }
+                    tmem_ld_wait();
                     float v[16];
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
@@ -198,6 +210,14 @@ gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                         unpack8(__ldg(reinterpret_cast<const uint4*>(p.bias + col0 + 8)), *reinterpret_cast<float(*)[8]>(b + 8));
 #pragma unroll
                         for (int j = 0; j < 16; ++j) v[j] += b[j];
+                    }
+                    if constexpr (kEpi) {
+                        float f[16];
+                        apply_act<16>(v, p.act);
+                        unpack8(res[0], *reinterpret_cast<float(*)[8]>(f));
+                        unpack8(res[1], *reinterpret_cast<float(*)[8]>(f + 8));
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] += f[j];
                     }
                     if (row_ok) {
                         asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -233,12 +253,13 @@ gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 
 // Host side: called by hkb_gemm_fp8_pts for M <= 64, batch == 1, N % 16 == 0 (arguments already validated).
 int launch_gemm_fp8_skinny(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias,
-                           int64_t M, int64_t N, int64_t K, uint32_t* status, cudaStream_t st) {
+                           const int* act, const void* residual, int64_t M, int64_t N, int64_t K, uint32_t* status, cudaStream_t st) {
     const int sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
     SkinnyParams p{};
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
     p.sa = sa; p.sb = sb; p.bias = (const __nv_bfloat16*)bias; p.C = (__nv_bfloat16*)C; p.status = status;
+    p.residual = (const __nv_bfloat16*)residual; p.act = act ? *act : HKB_ACT_NONE;
     p.a_box_rows = (int)((M + 7) / 8 * 8);
     p.a_bytes = (p.a_box_rows * 128 + 1023) / 1024 * 1024;
     const int units = (int)(N / 16);
@@ -263,9 +284,10 @@ int launch_gemm_fp8_skinny(const void* A, const void* B, void* C, const float* s
     rc = make_tmap_bytes(&tmB1, B, (uint64_t)K, (uint64_t)N, 1, (uint32_t)maxw * 16);
     if (rc != HKB_OK) return rc;
     // the limit is the kernel's, not the call's: every call sets the same one, whatever its own size (calls may overlap)
-    HKB_CUDA(cudaFuncSetAttribute(gemm_fp8_skinny_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    auto kern = act ? gemm_fp8_skinny_kernel<true> : gemm_fp8_skinny_kernel<false>;
+    HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
     const int grid = p.tiles < sms ? p.tiles : sms;
-    HKB_CUDA(launch_dependent(true, gemm_fp8_skinny_kernel, grid, 192, smem, 0, st, tmA, tmB0, tmB1, p));
+    HKB_CUDA(launch_dependent(true, kern, grid, 192, smem, 0, st, tmA, tmB0, tmB1, p));
     return check_launch("gemm_fp8_skinny_kernel");
 }
 

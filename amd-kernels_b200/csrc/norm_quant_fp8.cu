@@ -1,0 +1,258 @@
+// Residual addition + RMSNorm + FP8 (e4m3fn) quantization in one pass over the rows.
+//
+//   h = bf16(x + residual)                     the new residual stream, stored
+//   y = h * rsqrt(mean(h^2) + eps) * w         fp32, never stored
+//   scale = max(amax|y| / 448, 1e-10), q = e4m3fn_rne(clamp(y / scale, +-448)), amax over 128 columns or over the row
+//
+// h is rounded to bf16 before it is normalised, because the stored stream is what every later layer sees: the result is that of
+// an addition into the stream followed by the norm of the stream.  Sums, statistics and y stay in fp32.
+//
+// HBM bounds it: 2 + 2 bytes in and 2 + 1 out per element, and nothing is read twice, because a thread keeps its part of h in
+// registers from the sum to the codes.  A NaN, or an infinity in a row, comes out as the formula says: the maxima propagate NaN
+// into the scales (fmaxf would drop it and leave finite codes).
+#include "tc_common.cuh"
+
+namespace hkb {
+namespace {
+
+constexpr float kFp8Max = 448.0f;
+constexpr float kScaleFloor = 1e-10f;
+constexpr int kThreads = 256;
+
+// EL bf16 (8 or 16) of one row.  Plain loads, not the read-only path: residual_out may be x or residual.
+template <int EL> struct Chunk { uint32_t w[EL / 2]; };
+__device__ __forceinline__ void load(Chunk<16>& c, const __nv_bfloat16* p) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(c.w[0]), "=r"(c.w[1]), "=r"(c.w[2]), "=r"(c.w[3]), "=r"(c.w[4]), "=r"(c.w[5]), "=r"(c.w[6]), "=r"(c.w[7]) : "l"(p));
+}
+__device__ __forceinline__ void load(Chunk<8>& c, const __nv_bfloat16* p) {
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(c.w[0]), "=r"(c.w[1]), "=r"(c.w[2]), "=r"(c.w[3]) : "l"(p));
+}
+__device__ __forceinline__ void store(__nv_bfloat16* p, const Chunk<16>& c) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(c.w[0]), "r"(c.w[1]), "r"(c.w[2]), "r"(c.w[3]), "r"(c.w[4]), "r"(c.w[5]), "r"(c.w[6]), "r"(c.w[7]) : "memory");
+}
+__device__ __forceinline__ void store(__nv_bfloat16* p, const Chunk<8>& c) { *reinterpret_cast<uint4*>(p) = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]); }
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&o)[4]) { *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]); }
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&o)[2]) { *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]); }
+
+struct AddNormParams {
+    const __nv_bfloat16 *x, *residual, *w;
+    __nv_bfloat16* sum;
+    uint8_t* q;
+    float* scales;
+    int64_t M;
+    int D;
+    float eps;
+};
+
+// TPR threads share a row (256 / TPR rows per CTA), a thread holds NW chunks of EL elements, chunk index t + i * TPR.  The 128
+// columns of a scale group lie in 128 / EL neighbouring lanes of one i.  Rows of a CTA meet on their own named barrier only.
+template <int EL, int NW, int TPR, bool kRowScale>
+__global__ void __launch_bounds__(kThreads)
+add_rmsnorm_quant_kernel(const AddNormParams p) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int RPB = kThreads / TPR, WPR = TPR / 32;
+    const int tid = threadIdx.x, r_in = tid / TPR, t = tid % TPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + r_in;
+    const bool live = row < p.M;
+    const int chunks = p.D / EL;
+    const int64_t base = row * p.D;
+
+    __shared__ float s_part[2][kThreads / 32];
+    auto row_reduce = [&](int which, float v, auto op) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+        if constexpr (WPR > 1) {
+            if ((tid & 31) == 0) s_part[which][tid >> 5] = v;
+            if constexpr (TPR == kThreads) __syncthreads();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "r"(TPR) : "memory");
+            v = s_part[which][r_in * WPR];
+#pragma unroll
+            for (int k = 1; k < WPR; ++k) v = op(v, s_part[which][r_in * WPR + k]);
+        }
+        return v;
+    };
+
+    Chunk<EL> h[NW];
+    {
+        Chunk<EL> a[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int c = t + i * TPR;
+            if (live && c < chunks) {
+                load(a[i], p.x + base + (int64_t)c * EL);
+                load(h[i], p.residual + base + (int64_t)c * EL);
+            } else {
+#pragma unroll
+                for (int j = 0; j < EL / 2; ++j) a[i].w[j] = h[i].w[j] = 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+#pragma unroll
+            for (int j = 0; j < EL / 2; ++j) {
+                const float2 u = bf16x2_to_f2(a[i].w[j]), v = bf16x2_to_f2(h[i].w[j]);
+                const __nv_bfloat162 s = __floats2bfloat162_rn(u.x + v.x, u.y + v.y);
+                h[i].w[j] = *reinterpret_cast<const uint32_t*>(&s);
+            }
+    }
+    float2 ss2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const int c = t + i * TPR;
+        if (live && c < chunks) store(p.sum + base + (int64_t)c * EL, h[i]);
+#pragma unroll
+        for (int j = 0; j < EL / 2; ++j) { const float2 f = bf16x2_to_f2(h[i].w[j]); ss2 = __ffma2_rn(f, f, ss2); }
+    }
+    const float ss = row_reduce(0, ss2.x + ss2.y, [](float a, float b) { return a + b; });
+    const float rinv = rsqrtf(ss / (float)p.D + p.eps);
+    const float2 rinv2 = make_float2(rinv, rinv);
+
+    // y of chunk i, computed where it is needed: the gain comes from L1 / L2
+    auto normed = [&](int i, float2 (&y)[EL / 2]) {
+        const int c = t + i * TPR;
+        uint4 w[EL / 8];
+#pragma unroll
+        for (int k = 0; k < EL / 8; ++k)
+            w[k] = c < chunks ? __ldg(reinterpret_cast<const uint4*>(p.w + (int64_t)c * EL) + k) : make_uint4(0, 0, 0, 0);
+        const uint32_t* const ww = reinterpret_cast<const uint32_t*>(w);
+        float am = 0.0f;
+#pragma unroll
+        for (int j = 0; j < EL / 2; ++j) {
+            y[j] = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(h[i].w[j]), rinv2), bf16x2_to_f2(ww[j]));
+            am = max_nan(am, max_nan(fabsf(y[j].x), fabsf(y[j].y)));
+        }
+        return am;
+    };
+    // y is defined up to the order of the sum of squares, so the quotient is y * RN(1/scale), within one fp32 ulp of the division.
+    auto emit = [&](int i, const float2 (&y)[EL / 2], float rs) {
+        const int c = t + i * TPR;
+        const float2 rs2 = make_float2(rs, rs);
+        uint32_t o[EL / 4];
+#pragma unroll
+        for (int j = 0; j < EL / 4; ++j) {
+            const float2 qa = __fmul2_rn(y[2 * j], rs2), qb = __fmul2_rn(y[2 * j + 1], rs2);
+            o[j] = (uint32_t)cvt_e4m3x2(qa.x, qa.y) | ((uint32_t)cvt_e4m3x2(qb.x, qb.y) << 16);
+        }
+        if (live && c < chunks) store_codes(p.q + base + (int64_t)c * EL, o);
+    };
+
+    float2 y[EL / 2];
+    if constexpr (kRowScale) {
+        float am = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) am = max_nan(am, normed(i, y));
+        am = row_reduce(1, am, [](float a, float b) { return max_nan(a, b); });
+        const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor), rs = __frcp_rn(scale);
+        if (live && t == 0) p.scales[row] = scale;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            normed(i, y);
+            emit(i, y, rs);
+        }
+    } else {
+        constexpr int LANES = 128 / EL;
+        float* const sr = p.scales + row * (p.D / 128);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            float am = normed(i, y);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) am = max_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
+            const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor);
+            emit(i, y, __frcp_rn(scale));
+            const int c = t + i * TPR;
+            if (live && c < chunks && t % LANES == 0) sr[c / LANES] = scale;
+        }
+    }
+}
+
+template <int EL, int NW, bool kRowScale>
+int launch_add_norm(int tpr, const AddNormParams& p, cudaStream_t st) {
+    const unsigned grid = (unsigned)((p.M + kThreads / tpr - 1) / (kThreads / tpr));
+    auto kern = add_rmsnorm_quant_kernel<EL, NW, 256, kRowScale>;
+    if constexpr (EL * NW <= 64) {           // narrower teams hold at most 64 elements per thread
+        if (tpr == 32) kern = add_rmsnorm_quant_kernel<EL, NW, 32, kRowScale>;
+        if (tpr == 64) kern = add_rmsnorm_quant_kernel<EL, NW, 64, kRowScale>;
+        if (tpr == 128) kern = add_rmsnorm_quant_kernel<EL, NW, 128, kRowScale>;
+    }
+    HKB_CUDA(launch_dependent(true, kern, grid, kThreads, 0, 0, st, p));
+    return check_launch("add_rmsnorm_quant_kernel");
+}
+
+template <int EL, bool kRowScale>
+int dispatch_add_norm(const AddNormParams& p, cudaStream_t st) {
+    const int chunks = p.D / EL;
+    const int sms = sm_count();
+    HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
+    // 64 elements per thread, as in the other row quantizers; with few rows as many threads per row as there are chunks.
+    int tpr = 32;
+    while (tpr < 256 && (tpr * 64 < p.D || (tpr < chunks && p.M * tpr < (int64_t)kThreads * sms))) tpr *= 2;
+    const int n = (chunks + tpr - 1) / tpr;
+    if (n <= 1) return launch_add_norm<EL, 1, kRowScale>(tpr, p, st);
+    if (n <= 2) return launch_add_norm<EL, 2, kRowScale>(tpr, p, st);
+    if (n <= 4) return launch_add_norm<EL, 4, kRowScale>(tpr, p, st);
+    if constexpr (EL == 8) {
+        if (n > 8) return launch_add_norm<EL, 16, kRowScale>(tpr, p, st);
+    }
+    return launch_add_norm<EL, 8, kRowScale>(tpr, p, st);        // D <= 32768: n <= 8 chunks of 16, n <= 16 of 8
+}
+
+// fp32 groups of 128 -> codes and scales: eight lanes per group, 16 elements each.
+__global__ void __launch_bounds__(kThreads)
+quant_f32_1x128_kernel(const float* __restrict__ y, uint8_t* __restrict__ q, float* __restrict__ scales, int64_t groups) {
+    pdl_trigger();
+    pdl_wait();
+    const int64_t g = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / 8;
+    const int sub = threadIdx.x & 7;
+    float v[16];
+    float am = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float4 f = g < groups ? *reinterpret_cast<const float4*>(y + g * 128 + sub * 16 + 4 * k) : make_float4(0, 0, 0, 0);
+        v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) am = max_nan(am, fabsf(v[k]));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) am = max_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
+    const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor), rs = __frcp_rn(scale);
+    if (g < groups) {
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            o[k] = (uint32_t)cvt_e4m3x2(v[4 * k] * rs, v[4 * k + 1] * rs) | ((uint32_t)cvt_e4m3x2(v[4 * k + 2] * rs, v[4 * k + 3] * rs) << 16);
+        *reinterpret_cast<uint4*>(q + g * 128 + sub * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        if (sub == 0) scales[g] = scale;
+    }
+}
+
+}  // namespace
+
+int launch_quant_f32_1x128(const float* y, void* q, float* scales, int64_t groups, cudaStream_t st) {
+    HKB_CUDA(launch_dependent(true, quant_f32_1x128_kernel, (unsigned)((groups * 8 + kThreads - 1) / kThreads), kThreads, 0, 0, st, y, (uint8_t*)q, scales, groups));
+    return check_launch("quant_f32_1x128_kernel");
+}
+
+}  // namespace hkb
+
+extern "C" int hkb_add_rmsnorm_quant_fp8(const void* x, const void* residual, const void* w, void* q, float* scales, void* residual_out,
+                                         int64_t M, int64_t D, int64_t group, float eps, void* stream) {
+    using namespace hkb;
+    HKB_REQUIRE(x && residual && w && q && scales && residual_out, HKB_ERR_BAD_ARG, "add_rmsnorm_quant_fp8: null pointer");
+    HKB_REQUIRE(M >= 0 && M <= 0x7FFFFFFFLL && D > 0 && D <= 32768 && D % 8 == 0, HKB_ERR_BAD_SHAPE,
+                "add_rmsnorm_quant_fp8: need D %% 8 == 0 and 0 < D <= 32768, got M=%lld D=%lld", (long long)M, (long long)D);
+    HKB_REQUIRE(group == D || (group == 128 && D % 128 == 0), HKB_ERR_BAD_SHAPE,
+                "add_rmsnorm_quant_fp8: one scale per 128 columns (D %% 128 == 0) or per row, got group %lld of D=%lld", (long long)group, (long long)D);
+    HKB_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(residual_out) && ((uintptr_t)q & 7) == 0 && ((uintptr_t)scales & 3) == 0,
+                HKB_ERR_BAD_ALIGN, "add_rmsnorm_quant_fp8: x, residual, w and residual_out must be 16-byte, q 8-byte, scales 4-byte aligned");
+    if (M == 0) return HKB_OK;
+    const AddNormParams p{(const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)w, (__nv_bfloat16*)residual_out,
+                          (uint8_t*)q, scales, M, (int)D, eps};
+    // 32-byte chunks where every row of every tensor starts on one
+    const bool wide = D % 16 == 0 && aligned32(x) && aligned32(residual) && aligned32(residual_out) && aligned16(q);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (group == D) return wide ? dispatch_add_norm<16, true>(p, st) : dispatch_add_norm<8, true>(p, st);
+    return wide ? dispatch_add_norm<16, false>(p, st) : dispatch_add_norm<8, false>(p, st);
+}

@@ -264,6 +264,27 @@ int mxfp4_mode(const py::object& mode) {
     check(hkb_quant_fp8_1x128(x.ptr, w.none ? nullptr : w.ptr, q.ptr, (float*)s.ptr, M, D, eps, L.stream));
 }
 
+// Not in the reference: residual addition, RMSNorm and FP8 quantization in one pass.  residual_out (the new residual stream) may
+// be residual itself; scales [M, D/128] = one per 128 columns, [M] or [M, 1] = one per row.
+[[maybe_unused]] void fused_add_rmsnorm_fp8_quant_fwd(py::object input, py::object residual, py::object weight, py::object output,
+                                                      py::object scales, py::object residual_out, float eps) {
+    TView x = view(input, "input"), r = view(residual, "residual"), w = view(weight, "weight"), q = view(output, "output"),
+          s = view(scales, "scales"), h = view(residual_out, "residual_out");
+    for (const TView* t : {&x, &r, &w, &h}) want_dtype(*t, t->name, {"bfloat16"});
+    want_dtype(q, "output", {"float8_e4m3fn", "uint8"});
+    want_dtype(s, "scales", {"float32"});
+    if (x.rank() != 2) fail("input must be [M, D]");
+    const int64_t M = x.dim(0), D = x.dim(1);
+    if (r.numel != M * D || h.numel != M * D) fail("residual and residual_out must have M*D elements");
+    if (w.numel != D) fail("weight must have D elements");
+    if (q.numel != M * D) fail("output must have M*D elements");
+    const bool per_block = D % 128 == 0 && s.numel == M * (D / 128);
+    if (!per_block && s.numel != M) fail("scales must have M*(D/128) elements (one per 128 columns) or M (one per row)");
+    same_device({&x, &r, &w, &q, &s, &h});
+    Launch L(x.device);
+    check(hkb_add_rmsnorm_quant_fp8(x.ptr, r.ptr, w.ptr, q.ptr, (float*)s.ptr, h.ptr, M, D, per_block ? 128 : D, eps, L.stream));
+}
+
 // Not in the reference: 128x128 block quantizer that produces the weight operand and the
 // transposed b_scale [K/128, N/128] the block-scale GEMM consumes.
 [[maybe_unused]] void weight_quant_128x128(py::object weight, py::object output, py::object scales) {
@@ -334,6 +355,7 @@ struct GemmDims { int64_t batch, M, N, K; };
 // (the reference pads every tensor to 4-D with leading ones).
 GemmDims gemm_dims(const TView& A, const TView& B, const TView& C, int k_per_byte_num, int k_per_byte_den) {
     if (A.rank() < 2 || B.rank() < 2 || C.rank() < 2) fail("A, B, C must have at least 2 dimensions");
+    if (A.numel == 0 || B.numel == 0) fail("A and B must not be empty");
     GemmDims d;
     d.M = A.dim(-2);
     d.K = A.dim(-1) * k_per_byte_num / k_per_byte_den;
@@ -397,12 +419,45 @@ void fp8_pts(py::object A_, py::object B_, py::object C_, py::object sa_, py::ob
     check(hkb_gemm_fp8_ptgq(A.ptr, B.ptr, (const float*)bs.ptr, C.ptr, bias.none ? nullptr : bias.ptr, d.batch, d.M, d.N, d.K, L.stream));
 }
 
+// Activation names of the fused epilogues.
+int activation(const py::object& act) {
+    static const struct { const char* name; int id; } table[] = {{"none", HKB_ACT_NONE}, {"relu", HKB_ACT_RELU}, {"gelu", HKB_ACT_GELU},
+                                                                 {"gelu_tanh", HKB_ACT_GELU_TANH}, {"silu", HKB_ACT_SILU}};
+    if (act.is_none()) return HKB_ACT_NONE;
+    const std::string s = py::str(act).cast<std::string>();
+    for (const auto& e : table)
+        if (s == e.name) return e.id;
+    fail("unknown activation '" + s + "' (want 'none', 'relu', 'gelu', 'gelu_tanh' or 'silu')");
+}
+
+// Not in the reference: C = act(gemm + bias) + residual, per-token scales.  C may be residual itself.
+[[maybe_unused]] void dispatch_per_token_epilogue(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object bias_,
+                                                  py::object act_, py::object res_) {
+    TView A = view(A_, "A"), B = view(B_, "B"), C = view(C_, "C"), sa = view(sa_, "a_scale"), sb = view(sb_, "b_scale"),
+          bias = view(bias_, "bias", true), res = view(res_, "residual", true);
+    want_dtype(A, "A", {"float8_e4m3fn", "uint8"});
+    want_dtype(B, "B", {"float8_e4m3fn", "uint8"});
+    want_dtype(C, "C", {"bfloat16"});
+    want_dtype(sa, "a_scale", {"float32"});
+    want_dtype(sb, "b_scale", {"float32"});
+    for (const TView* t : {&bias, &res})
+        if (!t->none) want_dtype(*t, t->name, {"bfloat16"});
+    GemmDims d = gemm_dims(A, B, C, 1, 1);
+    if (sa.numel != d.batch * d.M) fail("a_scale must have batch*M elements");
+    if (sb.numel != d.batch * d.N) fail("b_scale must have batch*N elements");
+    if (!bias.none && bias.numel != d.batch * d.N) fail("bias must have batch*N elements");
+    if (!res.none && res.numel != d.batch * d.M * d.N) fail("residual must be [batch, M, N]");
+    const int act = activation(act_);
+    same_device({&A, &B, &C, &sa, &sb, &bias, &res});
+    Launch L(A.device);
+    check(hkb_gemm_fp8_pts_epilogue(A.ptr, B.ptr, C.ptr, (const float*)sa.ptr, (const float*)sb.ptr, bias.none ? nullptr : bias.ptr, act,
+                                    res.none ? nullptr : res.ptr, d.batch, d.M, d.N, d.K, L.stream));
+}
+
 // gemm_a8w8_blockscale_tk.dispatch(A, B, C, a_scale, b_scale):
 // kernels/gemm-basic/gemm_a8w8_blockscale/kernel.cpp:174-180.
 // a_scale [M, K/128]; b_scale [K/128, N/gn], gn = N / b_scale.shape[1] in {1, 128}.
-void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object ca_, py::object cb_) {
-    TView A = view(A_, "A"), B = view(B_, "B"), C = view(C_, "C"), sa = view(sa_, "a_scale"), sb = view(sb_, "b_scale"),
-          ca = view(ca_, "c_a", true), cb = view(cb_, "c_b", true);
+GemmDims blockscale_dims(const TView& A, const TView& B, const TView& C, const TView& sa, const TView& sb) {
     want_dtype(A, "A", {"float8_e4m3fn", "uint8"});
     want_dtype(B, "B", {"float8_e4m3fn", "uint8"});
     want_dtype(C, "C", {"bfloat16"});
@@ -411,13 +466,23 @@ void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py:
     GemmDims d = gemm_dims(A, B, C, 1, 1);
     if (d.batch != 1) fail("block-scale GEMM takes 2-D operands");
     if (d.K % 128) fail("K must be a multiple of 128");
+    if (sa.numel != d.M * (d.K / 128)) fail("a_scale must be [M, K/128]");
+    return d;
+}
+int64_t blockscale_gn(const GemmDims& d, const TView& sb) {
     const int64_t kb = d.K / 128;
-    if (sa.numel != d.M * kb) fail("a_scale must be [M, K/128]");
     if (sb.numel % kb) fail("b_scale must be [K/128, N/gn]");
     const int64_t ncols = sb.numel / kb;
     if (ncols == 0 || d.N % ncols) fail("b_scale must be [K/128, N/gn]");
     const int64_t gn = d.N / ncols;
     if (gn != 1 && gn != 128) fail("b_scale group size along N must be 1 or 128, got " + std::to_string(gn));
+    return gn;
+}
+void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object ca_, py::object cb_) {
+    TView A = view(A_, "A"), B = view(B_, "B"), C = view(C_, "C"), sa = view(sa_, "a_scale"), sb = view(sb_, "b_scale"),
+          ca = view(ca_, "c_a", true), cb = view(cb_, "c_b", true);
+    const GemmDims d = blockscale_dims(A, B, C, sa, sb);
+    const int64_t gn = blockscale_gn(d, sb);
     if (ca.none != cb.none) fail("c_a and c_b go together");
     if (!ca.none) {
         want_dtype(ca, "c_a", {"bfloat16"});
@@ -431,6 +496,53 @@ void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py:
     else
         check(hkb_gemm_fp8_blockscale_mul_add(A.ptr, B.ptr, C.ptr, (const float*)sa.ptr, (const float*)sb.ptr, gn, ca.ptr, cb.ptr,
                                               d.M, d.N, d.K, L.stream));
+}
+// Not in the reference: C = act(gemm + bias) + residual, block scales.  C may be residual itself.
+[[maybe_unused]] void dispatch_blockscale_epilogue(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object bias_,
+                                                   py::object act_, py::object res_) {
+    TView A = view(A_, "A"), B = view(B_, "B"), C = view(C_, "C"), sa = view(sa_, "a_scale"), sb = view(sb_, "b_scale"),
+          bias = view(bias_, "bias", true), res = view(res_, "residual", true);
+    const GemmDims d = blockscale_dims(A, B, C, sa, sb);
+    const int64_t gn = blockscale_gn(d, sb);
+    for (const TView* t : {&bias, &res})
+        if (!t->none) want_dtype(*t, t->name, {"bfloat16"});
+    if (!bias.none && bias.numel != d.N) fail("bias must have N elements");
+    if (!res.none && res.numel != d.M * d.N) fail("residual must be [M, N]");
+    const int act = activation(act_);
+    same_device({&A, &B, &C, &sa, &sb, &bias, &res});
+    Launch L(A.device);
+    check(hkb_gemm_fp8_blockscale_epilogue(A.ptr, B.ptr, C.ptr, (const float*)sa.ptr, (const float*)sb.ptr, gn, bias.none ? nullptr : bias.ptr, act,
+                                           res.none ? nullptr : res.ptr, d.M, d.N, d.K, L.stream));
+}
+// Not in the reference: gate and up projection (B [2F, K], gate rows first) and act(gate) * up in one GEMM.  C bf16 [M, F], or with
+// c_scale [M, F/128] e4m3fn codes.
+[[maybe_unused]] void dispatch_blockscale_gated(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object cs_,
+                                                py::object act_) {
+    TView A = view(A_, "A"), B = view(B_, "B"), C = view(C_, "C"), sa = view(sa_, "a_scale"), sb = view(sb_, "b_scale"), cs = view(cs_, "c_scale", true);
+    want_dtype(A, "A", {"float8_e4m3fn", "uint8"});
+    want_dtype(B, "B", {"float8_e4m3fn", "uint8"});
+    if (cs.none) want_dtype(C, "C", {"bfloat16"});
+    else want_dtype(C, "C", {"float8_e4m3fn", "uint8"});
+    want_dtype(sa, "a_scale", {"float32"});
+    want_dtype(sb, "b_scale", {"float32"});
+    if (!cs.none) want_dtype(cs, "c_scale", {"float32"});
+    if (A.rank() != 2 || B.rank() != 2 || C.rank() != 2 || A.dim(1) != B.dim(1)) fail("A [M, K], B [2F, K] and C [M, F] must be 2-D, A and B with the same K");
+    const int64_t M = A.dim(0), K = A.dim(1), F = C.dim(1);
+    if (C.dim(0) != M || B.dim(0) != 2 * F) fail("C must be [M, F] and B [2F, K] (the gate projection's rows, then the up projection's)");
+    if (K % 128 || F % 128) fail("K and F must be multiples of 128");
+    if (sa.numel != M * (K / 128)) fail("a_scale must be [M, K/128]");
+    if (sb.numel != (K / 128) * (2 * F / 128)) fail("b_scale must be [K/128, 2F/128]");
+    if (!cs.none && cs.numel != M * (F / 128)) fail("c_scale must be [M, F/128]");
+    const int act = activation(act_);
+    same_device({&A, &B, &C, &sa, &sb, &cs});
+    Launch L(A.device);
+    // the workspace is torch's, so that its life follows the stream (or the captured graph) that uses it
+    const int64_t bytes = hkb_gemm_fp8_blockscale_gated_workspace(M, F, K, cs.none ? 0 : 1);
+    if (bytes < 0) check((int)bytes);
+    py::object ws;
+    if (bytes > 0) ws = cs_.attr("new_empty")(bytes / 4);
+    check(hkb_gemm_fp8_blockscale_gated(A.ptr, B.ptr, C.ptr, cs.none ? nullptr : (float*)cs.ptr, (const float*)sa.ptr, (const float*)sb.ptr, act,
+                                        ws ? reinterpret_cast<void*>(ws.attr("data_ptr")().cast<uint64_t>()) : nullptr, M, F, K, L.stream));
 }
 [[maybe_unused]] void dispatch_blockscale(py::object A, py::object B, py::object C, py::object sa, py::object sb) {
     blockscale(A, B, C, sa, sb, py::none(), py::none());
@@ -756,8 +868,10 @@ PYBIND11_MODULE(HKB_SHIM_NAME, m) {
     m.doc() = "per-token dynamic quantization (FP8 e4m3fn, or INT8 when output is int8), sm_100a";
     m.def("per_token_quant_fwd", &per_token_quant_fwd, "input"_a, "output"_a, "scales"_a);
 #elif defined(HKB_SHIM_FUSED_FP8_QUANT)
-    m.doc() = "1x128 block FP8 quantizer with optional fused RMSNorm; 128x128 weight quantizer, sm_100a";
+    m.doc() = "1x128 block FP8 quantizer with optional fused RMSNorm, with residual addition also per row; 128x128 weight quantizer, sm_100a";
     m.def("fused_rmsnorm_fp8_quant_fwd", &fused_rmsnorm_fp8_quant_fwd, "input"_a, "weight"_a, "output"_a, "scales"_a, "eps"_a = 1e-6f);
+    m.def("fused_add_rmsnorm_fp8_quant_fwd", &fused_add_rmsnorm_fp8_quant_fwd, "input"_a, "residual"_a, "weight"_a, "output"_a,
+          "scales"_a, "residual_out"_a, "eps"_a = 1e-6f);
     m.def("weight_quant_128x128", &weight_quant_128x128, "weight"_a, "output"_a, "scales"_a);
 #elif defined(HKB_SHIM_FUSED_MXFP4_QUANT)
     m.doc() = "MXFP4 (e2m1 + e8m0 per 32) quantizer with optional fused RMSNorm, sm_100a";
@@ -771,9 +885,14 @@ PYBIND11_MODULE(HKB_SHIM_NAME, m) {
 #elif defined(HKB_SHIM_GEMM_A8W8_PER_TOKEN_SCALE)
     m.doc() = "FP8 GEMM with per-token / per-channel scales, sm_100a tcgen05";
     m.def("dispatch", &dispatch_per_token, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a);
+    m.def("dispatch_epilogue", &dispatch_per_token_epilogue, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a, "bias"_a = py::none(),
+          "activation"_a = "none", "residual"_a = py::none());
 #elif defined(HKB_SHIM_GEMM_A8W8_BLOCKSCALE)
     m.doc() = "FP8 GEMM with 1x128 activation and 128x128 (or 128x1) weight block scales, sm_100a tcgen05";
     m.def("dispatch", &dispatch_blockscale, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a);
+    m.def("dispatch_epilogue", &dispatch_blockscale_epilogue, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a, "bias"_a = py::none(),
+          "activation"_a = "none", "residual"_a = py::none());
+    m.def("dispatch_gated", &dispatch_blockscale_gated, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a, "c_scale"_a = py::none(), "activation"_a = "silu");
     m.def("dispatch_scatter", &dispatch_blockscale_scatter, "A"_a, "B"_a, "dst_ptrs"_a, "ldc"_a, "a_scale"_a, "b_scale"_a);
     m.def("dispatch_timeline", &dispatch_blockscale_timeline, "A"_a, "B"_a, "C"_a, "a_scale"_a, "b_scale"_a, "trace"_a);
 #elif defined(HKB_SHIM_GEMM_AFP4WFP4)

@@ -19,13 +19,27 @@ int make_tmap_bytes(CUtensorMap* map, const void* base, uint64_t row_bytes, uint
 int make_tmap_linear1k(CUtensorMap* map, const void* base, uint64_t bytes);
 
 // Per-token-scale FP8 GEMM for M <= 64, batch 1, N % 16 == 0 (gemm_fp8_skinny.cu); arguments are
-// expected to be validated by the caller.  `status` is the device status word.
+// expected to be validated by the caller.  act_or_null: C = act(gemm + bias) + residual.  `status` is the device status word.
 int launch_gemm_fp8_skinny(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* bias,
-                           int64_t M, int64_t N, int64_t K, uint32_t* status, cudaStream_t st);
+                           const int* act_or_null, const void* residual, int64_t M, int64_t N, int64_t K, uint32_t* status, cudaStream_t st);
 
-// Block-scale FP8 GEMM for M <= 32, 128-column weight-scale groups (gemm_fp8_blockscale_skinny.cu); c_a / c_b or null.
-int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, void* C, const float* sa, const float* sb, const void* c_a, const void* c_b,
-                                      int64_t M, int64_t N, int64_t K, int64_t ldc, uint32_t* status, cudaStream_t st);
+// Block-scale FP8 GEMM for M <= 32, 128-column weight-scale groups (gemm_fp8_blockscale_skinny.cu).  One of: c_a * gemm + c_b
+// (both or neither null); epilogue: act(gemm + bias) + residual; gated: B [2N, K] holds gate and up rows, act(gate) * up, to `f32`
+// [M, N] instead of C where that is not null.
+struct BsSkinnyOut {
+    void* C;                  // bf16, row pitch ldc elements
+    int64_t ldc;
+    const void *c_a = nullptr, *c_b = nullptr;
+    bool epilogue = false, gated = false;
+    const void* bias = nullptr;
+    int act = 0;
+    const void* residual = nullptr;
+    float* f32 = nullptr;
+};
+int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, const float* sa, const float* sb, const BsSkinnyOut& out, int64_t M,
+                                      int64_t N, int64_t K, uint32_t* status, cudaStream_t st);
+// fp32 groups of 128 -> e4m3fn codes and scales by the 1x128 rule; launched behind the kernel that writes them (norm_quant_fp8.cu).
+int launch_quant_f32_1x128(const float* y, void* q, float* scales, int64_t groups, cudaStream_t st);
 
 // MXFP4 GEMM for M <= 64, batch 1, N % 16 == 0, C 32-byte aligned (gemm_mxfp4_skinny.cu); scales in either layout.
 int launch_gemm_mxfp4_skinny(const void* A, const void* B, void* C, const void* sfa, const void* sfb, bool sfa_tc, bool sfb_tc,

@@ -5,10 +5,13 @@ re-implemented for NVIDIA B200 (sm_100a) behind the same module and function nam
 
     hk.per_token_quant_fwd(x, q, scales)                        # FP8 e4m3fn, one scale per row
     hk.fused_rmsnorm_fp8_quant_fwd(x, None, q, scales, eps)     # 1x128 block scales
+    hk.fused_add_rmsnorm_fp8_quant_fwd(x, residual, weight, q, scales, residual, eps)
     hk.fused_rmsnorm_mxfp4_quant_fwd(x, None, codes, scales, eps)
     hk.gemm.a8w8_per_token.dispatch(A, B, C, a_scale, b_scale)
     hk.gemm.a8w8.dispatch(A, B, a_scale, b_scale, C)
     hk.gemm.a8w8_blockscale.dispatch(A, B, C, a_scale, b_scale)
+    hk.gemm.a8w8_blockscale.dispatch_gated(A, B_gate_up, C, a_scale, b_scale, c_scale, "silu")
+    hk.gemm.a8w8_blockscale.dispatch_epilogue(A, B, C, a_scale, b_scale, bias, "none", residual)   # a8w8_per_token too
     hk.gemm.afp4wfp4.dispatch(A, B, C, a_scales, b_scales)
     hk.batched_gemm.a8w8.dispatch(A, B, a_scale, b_scale, C, bias)
     hk.batched_gemm.afp4wfp4.dispatch(A, B, C, a_scales, b_scales)
@@ -121,6 +124,13 @@ def per_token_quant_fwd(*args, **kwargs):
 def fused_rmsnorm_fp8_quant_fwd(*args, **kwargs):
     """(input, weight_or_None, output [M,D], scales f32 [M,D/128], eps)."""
     return _call("fused_fp8_quant_tk", "fused_rmsnorm_fp8_quant_fwd", *args, **kwargs)
+
+
+def fused_add_rmsnorm_fp8_quant_fwd(*args, **kwargs):
+    """(input, residual, weight, output [M,D], scales, residual_out, eps) -- not in the reference: adds
+    ``input`` to the residual stream (``residual_out`` may be ``residual``), normalises the sum and
+    quantizes it with one scale per 128 columns (``scales`` f32 [M,D/128]) or per row ([M,1])."""
+    return _call("fused_fp8_quant_tk", "fused_add_rmsnorm_fp8_quant_fwd", *args, **kwargs)
 
 
 def fused_rmsnorm_mxfp4_quant_fwd(*args, **kwargs):

@@ -32,6 +32,13 @@ typedef enum {
 #define HKB_MXFP4_MODE_DOC 0    /* e = floor(log2 amax) - 2, nearest value, ties to smaller */
 #define HKB_MXFP4_MODE_KERNEL 1 /* the reference device code's variant (rounded amax, truncation) */
 
+/* activation of the fused GEMM epilogues */
+#define HKB_ACT_NONE 0
+#define HKB_ACT_RELU 1
+#define HKB_ACT_GELU 2      /* v * Phi(v), Phi the normal distribution function (erf form) */
+#define HKB_ACT_GELU_TANH 3 /* v/2 * (1 + tanh(sqrt(2/pi) * (v + 0.044715 v^3))) */
+#define HKB_ACT_SILU 4      /* v / (1 + exp(-v)) */
+
 /* ---- library ------------------------------------------------------------------------- */
 int hkb_version(void);
 const char* hkb_last_error(void);
@@ -111,6 +118,19 @@ int hkb_quant_fp8_128x128(const void* w, void* q, float* scales,
  *   kernels/quantization/fused_mxfp4_quant/kernel.cpp:71-169,172-249,301-314. */
 int hkb_quant_mxfp4(const void* x, const void* w_or_null, void* codes, void* scales,
                     int64_t M, int64_t D, float eps, int mode, void* stream);
+
+/* Residual addition, RMSNorm and FP8 quantization in one pass: h = bf16(x + residual) is written to
+ * residual_out, y = h * rsqrt(mean(h^2) + eps) * w (fp32) is quantized by the rule above with one scale per
+ * `group` columns: group = 128 (scales f32 [M, D/128], the block-scale GEMM's a_scale; D % 128 == 0) or
+ * group = D (scales f32 [M], the per-token GEMM's).  x, residual, residual_out bf16 [M, D]; w bf16 [D]; q u8
+ * [M, D].  residual_out may be residual or x itself (the stream updated in place); any other overlap of outputs
+ * with inputs is not allowed.  A NaN or an infinity in a row goes into its codes and scales as the formula says.
+ * D % 8 == 0, D <= 32768; x, residual, residual_out and w 16-byte, q 8-byte aligned (fast path: D % 16 == 0,
+ * x, residual and residual_out 32-byte and q 16-byte aligned).  No counterpart in the reference project, whose
+ * fused quantizers take no residual and whose fused_add_rmsnorm does not quantize. */
+int hkb_add_rmsnorm_quant_fp8(const void* x, const void* residual, const void* w, void* q, float* scales,
+                              void* residual_out, int64_t M, int64_t D, int64_t group, float eps,
+                              void* stream);
 
 /* ---- GEMMs (all "NT": A [M,K] and B [N,K] are K-contiguous; C [M,N] bf16) ------------- */
 
@@ -279,6 +299,33 @@ int hkb_moe_gemm_mxfp4(const void* A, const void* B, void* C, const void* A_mx_s
                        const int32_t* sorted_token_ids, const int32_t* expert_ids, int64_t tokens,
                        int64_t num_padded, int64_t E, int64_t N, int64_t K,
                        int64_t num_valid_tokens, int64_t top_k, int mul_routed_weight, void* stream);
+
+/* The per-token-scale and the block-scale GEMM with bias, activation and residual in the epilogue:
+ *   C = bf16( act(gemm + bias) + residual )
+ * gemm as in hkb_gemm_fp8_pts / hkb_gemm_fp8_blockscale with their requirements, everything in fp32 up to the one
+ * rounding.  bias bf16 [batch, N] (block-scale: [N]) and residual bf16 [batch, M, N] ([M, N]) may be NULL, both
+ * 16-byte aligned; act one of HKB_ACT_*.  C may be residual itself (the residual stream updated in place); any
+ * other overlap of C with an operand is not allowed.  No counterpart in the reference project (its fused
+ * epilogues are the multiply-add and the split-concatenate). */
+int hkb_gemm_fp8_pts_epilogue(const void* A, const void* B, void* C, const float* sa, const float* sb,
+                              const void* bias_or_null, int act, const void* residual_or_null, int64_t batch,
+                              int64_t M, int64_t N, int64_t K, void* stream);
+int hkb_gemm_fp8_blockscale_epilogue(const void* A, const void* B, void* C, const float* sa, const float* sb,
+                                     int64_t gn, const void* bias_or_null, int act, const void* residual_or_null,
+                                     int64_t M, int64_t N, int64_t K, void* stream);
+
+/* Both projections of a gated feed-forward layer in one block-scale GEMM (gn = 128): B [2F, K] holds the gate
+ * projection's F rows, then the up projection's; with P = A @ B^T as in hkb_gemm_fp8_blockscale,
+ *   Y[m, f] = act(P[m, f]) * P[m, F + f]        fp32
+ * c_scale NULL: C bf16 [M, F] = bf16(Y).  Else C u8 [M, F] receives e4m3fn codes and c_scale f32 [M, F/128] their
+ * scales by the 1x128 rule (max(amax / 448, 1e-10)): the down projection's A and a_scale.  Y is rounded once, to C.
+ * sb f32 [K/128, 2F/128].  F, K multiples of 128; A, B 16-byte, C 32-byte, workspace 16-byte aligned.  workspace:
+ * hkb_gemm_fp8_blockscale_gated_workspace(M, F, K, c_scale != NULL) bytes of device memory (NULL when that is 0, < 0
+ * for arguments that the call would refuse), written and read by this call alone.  No counterpart in the reference project. */
+int64_t hkb_gemm_fp8_blockscale_gated_workspace(int64_t M, int64_t F, int64_t K, int fp8_output);
+int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* c_scale_or_null, const float* sa,
+                                  const float* sb, int act, void* workspace_or_null, int64_t M, int64_t F, int64_t K,
+                                  void* stream);
 
 /* quant_moe_tk: wire formats of the MoE activation/weight casts.  Replace
  *   quant_moe_tk.downcast_to_static_fp8(x, y, scale, M, N)

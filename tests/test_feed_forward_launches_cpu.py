@@ -1,0 +1,73 @@
+"""CPU tier: which kernels and grids the feed-forward operators' calls come to, against the stand-in runtime (fake_cudart.c) in a
+process of its own, this file as the program.  Torch is not imported: its kernels would register with the stand-in first."""
+import ctypes
+import os
+import shutil
+import subprocess
+import sys
+
+from test_launches_cpu import HKB_ERR_CUDA, ROOT, Runtime
+
+i64, f32, i32 = ctypes.c_int64, ctypes.c_float, ctypes.c_int
+
+
+def check_launches():
+    rt = Runtime()
+    rt.lib.hkb_gemm_fp8_blockscale_gated_workspace.restype = i64
+    P = rt.p(8)
+
+    def launches(call, expect=0):
+        seen = []
+        rt.on_launch = lambda name, grid, smem, args: seen.append((name, grid, smem)) or 0
+        assert call() == expect, rt.lib.hkb_last_error()
+        return seen
+
+    def norm(M, D, group):
+        return lambda: rt.lib.hkb_add_rmsnorm_quant_fp8(*P[:6], i64(M), i64(D), i64(group), f32(1e-6), None)
+
+    def gated(M, F, K, fp8):
+        return lambda: rt.lib.hkb_gemm_fp8_blockscale_gated(P[0], P[1], P[2], P[3] if fp8 else None, P[4], P[5], i32(4), P[6], i64(M), i64(F), i64(K), None)
+
+    # every row has its threads: grid * (256 / TPR) rows, TPR wide enough for D
+    for M in (1, 2, 3, 147, 148, 149, 1000, 16384, 2147483647):
+        for D in (8, 128, 136, 512, 1024, 2048, 4096, 4104, 8192, 16384, 16392, 32768):
+            for group in {D, 128 if D % 128 == 0 else D}:
+                (name, grid, _), = launches(norm(M, D, group))
+                el, nw, tpr = (int(v) for v in name.split("add_rmsnorm_quant_kernelILi")[1].split("ELb")[0].split("ELi"))
+                assert el * nw * tpr >= D, (M, D, name)
+                assert grid * (256 // tpr) >= M and (grid - 1) * (256 // tpr) < M, (M, D, name, grid)
+                assert el == (16 if D % 16 == 0 else 8)
+    # gated: one launch, and a second one for a decode call's codes; shared memory within the limit
+    for F, K in ((128, 128), (1152, 4224), (14336, 4096), (28672, 8192)):
+        for M in (1, 16, 17, 32, 33, 128, 129, 4096):
+            for fp8 in (False, True):
+                seen = launches(gated(M, F, K, fp8))
+                assert len(seen) == (2 if fp8 and M <= 32 else 1), (M, F, K, fp8, seen)
+                assert all(smem <= 232448 for _, _, smem in seen)
+                assert seen[0][1] <= 148
+                if len(seen) == 2:
+                    assert seen[1][1] * 32 >= M * F // 128
+    # a failing launch is that call's error and leaves nothing pending
+    for call in (norm(4, 512, 128), gated(4, 256, 256, True), gated(300, 256, 256, True)):
+        rt.on_launch = lambda *_: 701
+        assert call() == HKB_ERR_CUDA and rt.fake.fake_pending() == 0
+        rt.on_launch = lambda *_: 0
+        assert call() == 0
+
+
+def test_launches(tmp_path):
+    import pytest
+    inc = "/usr/local/cuda/include"
+    gcc = shutil.which("gcc")
+    if gcc is None or not os.path.exists(os.path.join(inc, "cuda_runtime_api.h")):
+        pytest.skip("no C compiler or CUDA runtime headers")
+    so = str(tmp_path / "fake_cudart.so")
+    src = os.path.join(ROOT, "tests", "fake_cudart.c")
+    subprocess.run([gcc, "-std=gnu11", "-O1", "-shared", "-fPIC", "-I", inc, src, "-o", so], check=True, capture_output=True, text=True)
+    r = subprocess.run([sys.executable, os.path.abspath(__file__), "check_launches"], env={**os.environ, "LD_PRELOAD": so}, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+if __name__ == "__main__":
+    globals()[sys.argv[1]]()
