@@ -84,6 +84,10 @@ cudaError_t launch_dependent(bool early, void (*kern)(KArgs...), unsigned grid, 
 // 81.0 / 79.9.
 inline bool starts_early(int64_t tiles, int64_t workers) { return tiles <= 4 * workers; }
 
+// How many clusters of `cluster` CTAs of this kernel the current device holds at once (cached; 0 where it cannot say).  Sets the
+// kernel's shared-memory limit to `smem`, the one that its launches set.
+int max_clusters(const void* kern, int threads, int smem, int cluster);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Number of SMs of the current device (cached per device).

@@ -113,6 +113,7 @@ struct GemmParams {
     int skip_kblock;           // >= 0: the producer leaves this K block of its first tile unloaded (wait-limit probe only)
     const __nv_bfloat16* residual;   // kOut == 5: C = act(gemm + bias) + residual, [batch, M, N] or null
     int act;                   // kOut == 5, 6: HKB_ACT_*
+    int split;                 // kSplitK: CTAs (a cluster of 2, 4 or 8) that share a tile, each with a part of K
     uint8_t* q_out;            // kOut == 6: codes [M, N/2] and scales [M, N/256] instead of C, or null
     float* q_scale;
     unsigned long long* trace; // timeline build (kOut == 4) only: [grid][kTraceEvents][kTraceKb] SM clock readings
@@ -201,20 +202,33 @@ __device__ __forceinline__ void mul_add_cols(const __nv_bfloat16* c_a, const __n
 // Bias / activation / residual epilogue on NV consecutive columns of one row from `col` (a multiple of 8, all in range or, per 8
 // columns, all out).  load_residual() goes first, ahead of every store: C may be the residual, so the compiler cannot move the
 // loads up, and they are the one long latency of the epilogue.  Plain loads for the same reason.
-template <int NV>
-__device__ __forceinline__ void load_residual(const __nv_bfloat16* rrow, int col, int N, uint4 (&r)[NV / 8]) {
+// kTail: columns from N on do not exist.  Without it the loads are unconditional: behind a branch each they would wait for one
+// another.  `wide`: rows start on 32 bytes; a lane then takes a whole sector per load (half a sector per load reads each of them
+// twice, the lanes of a warp being in 32 different rows).
+template <int NV, bool kTail>
+__device__ __forceinline__ void load_residual(const __nv_bfloat16* rrow, int col, int N, bool wide, uint4 (&r)[NV / 8]) {
 #pragma unroll
-    for (int j = 0; j < NV / 8; ++j) {
-        r[j] = make_uint4(0, 0, 0, 0);
-        if (rrow && col + 8 * j < N) r[j] = *reinterpret_cast<const uint4*>(rrow + col + 8 * j);
+    for (int j = 0; j < NV / 8; ++j) r[j] = make_uint4(0, 0, 0, 0);
+    if (!rrow) return;
+    if (NV > 8 && wide) {
+#pragma unroll
+        for (int j = 0; j + 1 < NV / 8; j += 2)
+            if (!kTail || col + 8 * j < N)
+                asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                             : "=r"(r[j].x), "=r"(r[j].y), "=r"(r[j].z), "=r"(r[j].w), "=r"(r[j + 1].x), "=r"(r[j + 1].y), "=r"(r[j + 1].z), "=r"(r[j + 1].w)
+                             : "l"(rrow + col + 8 * j));
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV / 8; ++j)
+            if (!kTail || col + 8 * j < N) r[j] = *reinterpret_cast<const uint4*>(rrow + col + 8 * j);
     }
 }
 template <int NV>
-__device__ __forceinline__ void add_bias(const __nv_bfloat16* bias, int col, int N, float* v) {
+__device__ __forceinline__ void add_bias(const __nv_bfloat16* bias, int col, float* v) {
 #pragma unroll
     for (int j = 0; j < NV; j += 8) {
         float b[8];
-        unpack8(col + j < N ? __ldg(reinterpret_cast<const uint4*>(bias + col + j)) : make_uint4(0, 0, 0, 0), b);
+        unpack8(__ldg(reinterpret_cast<const uint4*>(bias + col + j)), b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[j + i] += b[i];
     }
@@ -290,7 +304,12 @@ constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 
 // the same output columns (two boxes, no re-ordering of the weights), and the tile gives BN/2 columns act(gate) * up.  A thread
 // promotes 64 gate and the 64 matching up columns, so the product needs nobody else; with FP8 output the two warps of a row
 // exchange one maximum through shared memory (BN = 256: a tile is exactly one 128-column scale group of the result).
-template <int BN, int STAGES, bool kBlockScale, bool kGn128, bool kPair = false, int AROWS = BM, int kOut = 0>
+// kSplitK (kOut 5 and 6): a cluster of p.split CTAs has exactly one tile, each CTA a part of K.  At the end every epilogue warp writes
+// its sums, a slice of its columns to each CTA of the cluster, into the operand rings (idle by then) through distributed shared
+// memory, and finishes its own slice: the parts added in the order of their ranks, so the result is the same every time, and every
+// warp of every CTA has a share of the epilogue.  The cluster barriers around that are reached by every thread on every path, an
+// abandoned wait included.  A template of its own: the same loop with the part's bounds in variables ran 4-6 % slower whole.
+template <int BN, int STAGES, bool kBlockScale, bool kGn128, bool kPair = false, int AROWS = BM, int kOut = 0, bool kSplitK = false>
 __global__ void __launch_bounds__(gemm_threads<BN, kBlockScale, kPair>(), 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p,
                 const __grid_constant__ CUtensorMap tmBHalf) {
@@ -300,6 +319,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     using L = SmemLayout<BN, STAGES, kPair, AROWS, (kBlockScale && kGn128) ? 128 * EPI_GROUPS : 0, kScaleChunk, kStageOut>;
     constexpr bool kGrouped = kOut == 3;
     constexpr bool kTrace = kOut == 4;
+    static_assert(!kSplitK || EPI_GROUPS * 4 * (BN / EPI_GROUPS) * 128 + (kOut == 6 ? 8 * 8 * 32 * 4 : 0) <= STAGES * L::kStageBytes, "split K: slots in the operand ring");
     constexpr bool kEpi = kOut == 5;
     constexpr bool kGated = kOut == 6;
     static_assert(!kGated || (kBlockScale && kGn128 && !kPair), "gated mode: block scales, 128-column groups, one CTA");
@@ -331,7 +351,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int kblocks = p.K / BK;
+    // split K: a cluster of p.split CTAs has exactly one tile, CTA `part` its K blocks [k_begin, k_begin + kblocks)
+    static_assert(!kSplitK || (!kPair && (kEpi || kGated) && (!kBlockScale || kGn128)), "split K: one CTA, an epilogue of its own");
+    const int all_kblocks = p.K / BK;
+    const int split = kSplitK ? p.split : 1;
+    const int part = kSplitK ? (int)cluster_ctarank() : 0;
+    const int k_begin = kSplitK ? all_kblocks * part / split : 0;
+    const int kblocks = kSplitK ? all_kblocks * (part + 1) / split - k_begin : all_kblocks;
     auto trace_at = [&](int ev, int kb, bool on, long long clk) {
         if constexpr (kTrace) {
             if (on && kb < kTraceKb) p.trace[((size_t)blockIdx.x * kTraceEvents + ev) * kTraceKb + kb] = (unsigned long long)clk;
@@ -348,8 +374,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int total_tiles = kSplit ? all_tiles + (all_tiles - p.split_from) : all_tiles;
     auto tile_of = [&](int v) { return kSplit && v >= p.split_from ? p.split_from + (v - p.split_from) / 2 : v; };
     auto half_of = [&](int v) { return kSplit && v >= p.split_from ? (v - p.split_from) & 1 : -1; };      // -1: the whole tile
-    const int tile0 = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
-    const int tile_step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+    const int tile0 = kPair ? (int)(blockIdx.x >> 1) : kSplitK ? (int)blockIdx.x / split : (int)blockIdx.x;
+    const int tile_step = kPair ? (int)(gridDim.x >> 1) : kSplitK ? (int)gridDim.x / split : (int)gridDim.x;
     constexpr int TILE_M = kPair ? 2 * BM : BM;
 
     if (threadIdx.x == 0) {
@@ -423,12 +449,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         else tma_load_3d_pair(sa + L::kABytes, &tmBHalf, full_bar(s), kb * BK, nb * BN + half * (BN / 2) + (int)rank * (L::kBRows / 2), b);
                     } else {
                         mbar_arrive_expect_tx(full_bar(s), stage_tx);
-                        tma_load_3d(sa, &tmA, full_bar(s), kb * BK, a_row, a_z);
+                        const int x = (k_begin + kb) * BK;
+                        tma_load_3d(sa, &tmA, full_bar(s), x, a_row, a_z);
                         if constexpr (kGated) {
-                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), kb * BK, nb * (BN / 2), 0);
-                            tma_load_3d(sa + L::kABytes + BN / 2 * BK, &tmB, full_bar(s), kb * BK, p.N / 2 + nb * (BN / 2), 0);
+                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), x, nb * (BN / 2), 0);
+                            tma_load_3d(sa + L::kABytes + BN / 2 * BK, &tmB, full_bar(s), x, p.N / 2 + nb * (BN / 2), 0);
                         } else {
-                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), kb * BK, nb * BN, b_z);
+                            tma_load_3d(sa + L::kABytes, &tmB, full_bar(s), x, nb * BN, b_z);
                         }
                     }
                     if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -548,9 +575,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             }
             if (r >= p.M) r = p.M - 1;
             const int kb0 = chunk * kScaleChunk;
-            const float* src = p.sa + (int64_t)r * kblocks + kb0;
+            const float* src = p.sa + (int64_t)r * all_kblocks + k_begin + kb0;
             const uint32_t dst = smem_u32(sa_slots + (size_t)buf * (kScaleChunk / 4) * EPI_THREADS);
-            const bool vec = (kblocks % 4) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
+            const bool vec = (kblocks % 4) == 0 && (k_begin % 4) == 0 && (all_kblocks % 4) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < kScaleChunk / 4; ++j) {
                 const int kb = kb0 + 4 * j;
@@ -567,10 +594,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const int kb = kb0 + lane;
             if (lane < kScaleChunk && kb < kblocks) {
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                             ::"r"(smem_u32(sb_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)kb * nsb + cg) : "memory");
+                             ::"r"(smem_u32(sb_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)(k_begin + kb) * nsb + cg) : "memory");
                 if constexpr (kGated)
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
-                                 ::"r"(smem_u32(sbu_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)kb * nsb + nsb / 2 + cg) : "memory");
+                                 ::"r"(smem_u32(sbu_slots + (size_t)buf * EPI_WARPS * kScaleChunk + lane)), "l"(sb_base + (int64_t)(k_begin + kb) * nsb + nsb / 2 + cg) : "memory");
             }
         };
         // grouped mode: the first tile at or after `t` (in this CTA's walk) that the tile list does not mark as empty
@@ -608,15 +635,114 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const int col_base = nb * BN + (half < 0 ? grp * COLS_PER_GROUP : half * (BN / 2) + grp * (COLS_PER_GROUP / 2));
             __nv_bfloat16* crow = p.C + ((int64_t)b * p.M + (row_ok ? row : 0)) * p.ldc;
             const __nv_bfloat16* rrow = kEpi && p.residual && row_ok ? p.residual + ((int64_t)b * p.M + row) * p.N : nullptr;
-            if constexpr (kEpi) {       // the row's residuals go towards L2 while the tile is computed
+            const bool res_wide = kEpi && (p.N % 16) == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 31) == 0;
+            // the row's residuals go towards L2 a few K blocks before they are needed (at the tile's start they would be gone again
+            // from L2 by its end, behind the operands of a long K)
+            auto prefetch_residual = [&]() {
                 if (rrow)
                     for (int c = 0; c < cols && col_base + c < p.N; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(rrow + col_base + c));
+            };
+            if constexpr (kEpi && !kBlockScale) prefetch_residual();
+            // ---- split K ----
+            // Slots in the operand rings: [rank of the sender][epilogue warp][16-byte chunk of the slice][lane].  A slice is COLS_PER_GROUP /
+            // split columns of the warp (gated: half as many gate columns, then the up columns that go with them).
+            const int nchunk = kSplitK ? COLS_PER_GROUP / 4 / split : 1;
+            const bool any_rows = mb * TILE_M + quarter * 32 < p.M;              // warp-uniform: rows that exist
+            auto cluster_meet = [&]() { __syncwarp(); cluster_sync_all(); };
+            auto send_part = [&](int j, float x0, float x1, float x2, float x3) {      // columns 4j .. 4j+3 of the warp's
+                const int run = kGated ? nchunk / 2 : nchunk, jj = kGated ? j % (COLS_PER_GROUP / 8) : j;
+                const int local = jj % run + (kGated && j >= COLS_PER_GROUP / 8 ? run : 0);
+                st_cluster4(cluster_addr(smem_base + (uint32_t)(((part * EPI_WARPS + ew) * nchunk + local) * 512 + lane * 16), jj / run), x0, x1, x2, x3);
+            };
+            auto sum_parts = [&](int chunk, float (&v)[8]) {                     // two chunks of this thread's slice, parts in rank order
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+                for (int r = 0; r < split; ++r) {
+                    const float4* const src = reinterpret_cast<const float4*>(smem + (uint32_t)(((r * EPI_WARPS + ew) * nchunk + chunk) * 512 + lane * 16));
+                    const float4 a = src[0], b4 = src[32];
+                    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                    v[4] += b4.x; v[5] += b4.y; v[6] += b4.z; v[7] += b4.w;
+                }
+            };
+            // kEpi: weight scales and bias of the slice, four columns per lane, are fetched ahead of the main loop and go round by shuffles
+            const int slice0 = col_base + part * (4 * nchunk);
+            float4 sl_sb = make_float4(1, 1, 1, 1);
+            uint2 sl_bias = make_uint2(0, 0);
+            float sl_sa = 1.0f;
+            if constexpr (kSplitK && kEpi) {
+                if (lane < nchunk && slice0 + 4 * lane < p.N) {
+                    if constexpr (!kBlockScale) sl_sb = __ldg(reinterpret_cast<const float4*>(p.sb + (int64_t)b * p.N + slice0 + 4 * lane));
+                    if (p.bias) sl_bias = __ldg(reinterpret_cast<const uint2*>(p.bias + (int64_t)b * p.N + slice0 + 4 * lane));
+                }
+                if (!kBlockScale && row_ok) sl_sa = __ldg(p.sa + (int64_t)b * p.M + row);
             }
-
+            auto finish_slice = [&]() {                                          // kEpi: bias, activation, residual, store
+                uint4 next[1];
+                load_residual<8, true>(rrow, slice0, p.N, false, next);
+                for (int i = 0; i < nchunk / 2; ++i) {
+                    const int col = slice0 + 8 * i;
+                    if (col >= p.N) break;                                       // uniform
+                    const uint4 res = next[0];
+                    if (i + 1 < nchunk / 2) load_residual<8, true>(rrow, col + 8, p.N, false, next);
+                    float v[8];
+                    sum_parts(2 * i, v);
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        const int from = 2 * i + j / 4;
+                        if constexpr (!kBlockScale) {
+                            v[j] = v[j] * sl_sa * __shfl_sync(0xFFFFFFFFu, sl_sb.x, from);
+                            v[j + 1] = v[j + 1] * sl_sa * __shfl_sync(0xFFFFFFFFu, sl_sb.y, from);
+                            v[j + 2] = v[j + 2] * sl_sa * __shfl_sync(0xFFFFFFFFu, sl_sb.z, from);
+                            v[j + 3] = v[j + 3] * sl_sa * __shfl_sync(0xFFFFFFFFu, sl_sb.w, from);
+                        }
+                        if (p.bias) {
+                            const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, sl_bias.x, from), b1 = __shfl_sync(0xFFFFFFFFu, sl_bias.y, from);
+                            v[j] += bf16_lo(b0); v[j + 1] += bf16_hi(b0); v[j + 2] += bf16_lo(b1); v[j + 3] += bf16_hi(b1);
+                        }
+                    }
+                    apply_act<8>(v, p.act);
+                    add_residual<8>(&res, v);
+                    if (row_ok) store_bf16x8(crow + col, v);
+                }
+            };
             if constexpr (!kBlockScale) {
                 const float sa = row_ok ? __ldg(p.sa + (int64_t)b * p.M + row) : 0.0f;
                 const float* sbp = p.sb + (int64_t)b * p.N;
                 const __nv_bfloat16* biasp = p.bias ? p.bias + (int64_t)b * p.N : nullptr;
+                // kEpi: scales and bias of the warp's columns, four per lane, are fetched while the tile is computed and go round by
+                // shuffles; the residuals are a 32-column step ahead.  With these loads inside the steps, each behind its own test, a
+                // step waited for memory four times over: 4096 x 4096 x 1024, us, plain epilogue 24.3 / 22.0, bias 25.5 / 23.8.  (Output turned
+                // through shared memory so that eight lanes store one row's 128 bytes: 24.1, 25.6, and gelu 42.8 instead of 32.)
+                float4 sb_own = make_float4(0, 0, 0, 0);
+                uint2 bias_own = make_uint2(0, 0);
+                uint4 res_next[4];
+                if constexpr (kEpi && !kSplitK) {
+                    const int own = col_base + 4 * lane;
+                    if (4 * lane < cols && own < p.N) {
+                        sb_own = __ldg(reinterpret_cast<const float4*>(sbp + own));
+                        if (biasp) bias_own = __ldg(reinterpret_cast<const uint2*>(biasp + own));
+                    }
+                    load_residual<32, true>(rrow, col_base, p.N, res_wide, res_next);
+                }
+                if constexpr (kSplitK) {
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar(acc), acc_ph, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns));
+                    tc_fence_after();
+                    cluster_meet();
+                    if (ok && any_rows) {
+#pragma unroll
+                        for (int c = 0; c < COLS_PER_GROUP; c += 32) {
+                            uint32_t r[32];
+                            tmem_ld32(tmem_base + lane_addr + grp * COLS_PER_GROUP + c, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                send_part(c / 4 + j, __uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                        }
+                    }
+                    cluster_meet();
+                    if (ok && any_rows) finish_slice();
+                    break;                                                       // the only tile of this cluster
+                }
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar(acc), acc_ph, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t t_addr = tmem_base + lane_addr + acc * BN + grp * cols;
@@ -625,8 +751,33 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     uint32_t r[32];
                     tmem_ld32(t_addr + c, r);
                     const int col0 = col_base + c;
-                    uint4 res[4];
-                    if constexpr (kEpi) load_residual<32>(rrow, col0, p.N, res);
+                    if constexpr (kEpi) {
+                        uint4 res[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) res[j] = res_next[j];
+                        if (c + 32 < cols) load_residual<32, true>(rrow, col0 + 32, p.N, res_wide, res_next);
+                        tmem_ld_wait();
+                        float w[32];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const int from = (c + j) >> 2;
+                            w[j] = __uint_as_float(r[j]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.x, from);
+                            w[j + 1] = __uint_as_float(r[j + 1]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.y, from);
+                            w[j + 2] = __uint_as_float(r[j + 2]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.z, from);
+                            w[j + 3] = __uint_as_float(r[j + 3]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.w, from);
+                        }
+                        if (biasp) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, bias_own.x, (c + j) >> 2), b1 = __shfl_sync(0xFFFFFFFFu, bias_own.y, (c + j) >> 2);
+                                w[j] += bf16_lo(b0); w[j + 1] += bf16_hi(b0); w[j + 2] += bf16_lo(b1); w[j + 3] += bf16_hi(b1);
+                            }
+                        }
+                        apply_act<32>(w, p.act);
+                        add_residual<32>(res, w);
+                        if (row_ok) store_row32(crow, col0, p.N, w, wide);
+                        continue;
+                    }
                     tmem_ld_wait();
                     float v[32];
 #pragma unroll
@@ -642,10 +793,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         }
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[j + i] = __uint_as_float(r[j + i]) * sa * sv[i] + bv[i];
-                    }
-                    if constexpr (kEpi) {
-                        apply_act<32>(v, p.act);
-                        add_residual<32>(res, v);
                     }
                     if (row_ok) store_row32(crow, col0, p.N, v, wide);
                 }
@@ -682,6 +829,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const int kb_end = min(kbs - ch * kScaleChunk, kScaleChunk);
                     float4 sa4 = sa_s[0];
                 for (int kk = 0; kk < kb_end; ++kk) {
+                    if constexpr (kEpi) {
+                        if (ch * kScaleChunk + kk == max(kbs - 6, 0)) prefetch_residual();
+                    }
                     const int sub = kk & 3;
                     const float sa_k = sub == 0 ? sa4.x : sub == 1 ? sa4.y : sub == 2 ? sa4.z : sa4.w;
                     const float sc = sa_k * sb_s[kk];
@@ -728,6 +878,59 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     if (++acc == 2) { acc = 0; acc_ph ^= 1; }
                 }
                     sbuf ^= 1;
+                }
+                if constexpr (kSplitK) {
+                    cluster_meet();
+                    if (ok && any_rows) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) send_part(j, acc2[2 * j].x, acc2[2 * j].y, acc2[2 * j + 1].x, acc2[2 * j + 1].y);
+                    }
+                    cluster_meet();
+                    if constexpr (kEpi) {
+                        if (ok && any_rows) finish_slice();
+                    } else {
+                        const int F = p.N / 2, outs = 64 / split, out0 = nb * (BN / 2) + grp * 64 + part * outs;
+                        auto gated8 = [&](int i, float (&y)[8]) {                // outputs 8i .. 8i+7 of this thread's slice
+                            float up[8];
+                            sum_parts(2 * i, y);
+                            sum_parts(outs / 4 + 2 * i, up);
+                            apply_act<8>(y, p.act);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) y[k] *= up[k];
+                        };
+                        const bool mine = ok && any_rows;
+                        if (BN == 256 && p.q_out) {
+                            // the row's maximum: every warp tells every CTA its own (behind the slots of the sums)
+                            float* const maxima = reinterpret_cast<float*>(smem + EPI_WARPS * COLS_PER_GROUP * 128);      // [rank][warp][lane]
+                            float am = 0.0f, y[8];
+                            if (mine)
+                                for (int i = 0; i < outs / 8; ++i) {
+                                    gated8(i, y);
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) am = max_nan(am, fabsf(y[k]));
+                                }
+                            for (int r = 0; r < split; ++r) st_cluster(cluster_addr(smem_u32(maxima + (part * EPI_WARPS + ew) * 32 + lane), r), am);
+                            cluster_meet();
+                            if (mine) {
+                                for (int r = 0; r < split; ++r) am = max_nan(am, max_nan(maxima[(r * EPI_WARPS + ew) * 32 + lane], maxima[(r * EPI_WARPS + (ew ^ 4)) * 32 + lane]));
+                                const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f), rs = __frcp_rn(scale);
+                                for (int i = 0; i < outs / 8; ++i) {
+                                    gated8(i, y);
+                                    const uint2 o = make_uint2((uint32_t)cvt_e4m3x2(y[0] * rs, y[1] * rs) | ((uint32_t)cvt_e4m3x2(y[2] * rs, y[3] * rs) << 16),
+                                                               (uint32_t)cvt_e4m3x2(y[4] * rs, y[5] * rs) | ((uint32_t)cvt_e4m3x2(y[6] * rs, y[7] * rs) << 16));
+                                    if (row_ok) *reinterpret_cast<uint2*>(p.q_out + (int64_t)row * F + out0 + 8 * i) = o;
+                                }
+                                if (row_ok && grp == 0 && part == 0) p.q_scale[(int64_t)row * (F / 128) + nb] = scale;
+                            }
+                        } else if (mine) {
+                            for (int i = 0; i < outs / 8; ++i) {
+                                float y[8];
+                                gated8(i, y);
+                                if (row_ok) store_bf16x8(p.C + (int64_t)row * F + out0 + 8 * i, y);
+                            }
+                        }
+                    }
+                    break;                                                       // the only tile of this cluster
                 }
                 if constexpr (kOut == 1) {
                     // Scatter mode: the copies in the other GPUs' memory travel over NVLink, where a 32-byte store per
@@ -807,13 +1010,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                         for (int h = 0; h < 128; h += 64) {      // all residuals of 64 columns are in flight at once; 128 do not fit the registers
                             uint4 res[8];
-                            load_residual<64>(rrow, col_base + h, p.N, res);
+                            load_residual<64, false>(rrow, col_base + h, p.N, res_wide, res);
 #pragma unroll
                             for (int c = 0; c < 64; c += 16) {
                                 float v[16];
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) { v[2 * i] = acc2[(h + c) / 2 + i].x; v[2 * i + 1] = acc2[(h + c) / 2 + i].y; }
-                                if (p.bias) add_bias<16>(p.bias, col_base + h + c, p.N, v);
+                                if (p.bias) add_bias<16>(p.bias, col_base + h + c, v);
                                 apply_act<16>(v, p.act);
                                 add_residual<16>(res + c / 8, v);
                                 store_bf16x16(crow + col_base + h + c, v);
@@ -881,8 +1084,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                     for (int c = 0; c < COLS_PER_GROUP; c += 32) {
                         uint4 res[4];
-                        load_residual<32>(rrow, col_base + c, p.N, res);
-                        if (p.bias) add_bias<32>(p.bias, col_base + c, p.N, accv + c);
+                        load_residual<32, false>(rrow, col_base + c, p.N, res_wide, res);
+                        if (p.bias) add_bias<32>(p.bias, col_base + c, accv + c);
                         apply_act<32>(accv + c, p.act);
                         add_residual<32>(res, accv + c);
                         store_row32(crow, col_base + c, p.N, accv + c, wide);
@@ -904,6 +1107,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
 
     // ---- teardown: every role is done (or has given up); free TMEM ----
+    if constexpr (kSplitK) {
+        if (warp < EPI_WARP0) {         // the epilogue warps' cluster barriers, reached by everyone
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
+            if (kGated && BN == 256 && p.q_out) cluster_sync_all();
+        }
+    }
     asm volatile("cp.async.wait_group 0;" ::: "memory");      // no staged-scale copy may outlive the CTA
     tc_fence_before();
     __syncthreads();
@@ -1001,18 +1212,23 @@ inline bool skinny_enabled() {
     return on;
 }
 
-template <int BN, int STAGES, bool kBlockScale, bool kGn128 = false, int AROWS = BM, int kOut = 0>
+template <int BN, int STAGES, bool kBlockScale, bool kGn128 = false, int AROWS = BM, int kOut = 0, bool kSplitK = false>
 int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p, cudaStream_t st) {
     using L = SmemLayout<BN, STAGES, false, AROWS, (kBlockScale && kGn128) ? (BN == 256 ? 256 : 128) : 0, kOut == 1 ? 16 : 32, stage_out_bytes<BN, kOut>()>;
     static_assert(L::kDynamic <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
-    auto kern = gemm_fp8_kernel<BN, STAGES, kBlockScale, kGn128, false, AROWS, kOut>;
+    auto kern = gemm_fp8_kernel<BN, STAGES, kBlockScale, kGn128, false, AROWS, kOut, kSplitK>;
     // the attribute is per device; set it on every call (cheap) so multi-device processes work
     HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic));
     const int tiles = p.m_blks * p.n_blks * p.batch;
     const int sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
-    const int grid = tiles < sms ? tiles : sms;
-    HKB_CUDA(launch_dependent(starts_early(tiles, grid), kern, grid, gemm_threads<BN, kBlockScale>(), L::kDynamic, 0, st, tmA, tmB, p, tmB));
+    const int grid = kSplitK ? tiles * p.split : tiles < sms ? tiles : sms;
+    HKB_CUDA(launch_dependent(starts_early(tiles, grid), kern, grid, gemm_threads<BN, kBlockScale>(), L::kDynamic, kSplitK ? p.split : 0, st, tmA, tmB, p, tmB));
+    if (kSplitK)
+        note_kernel(kOut == 5 ? (kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,epilogue,split>" : "gemm_fp8_kernel<128,blockscale,epilogue,split>")
+                                             : (BN == 128 ? "gemm_fp8_kernel<128,pts,epilogue,split>" : "gemm_fp8_kernel<64,pts,epilogue,split>"))
+                              : (BN == 256 ? "gemm_fp8_kernel<256,blockscale,gated,split>" : "gemm_fp8_kernel<128,blockscale,gated,split>"));
+    else
     note_kernel(kOut == 1 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,scatter>" : "gemm_fp8_kernel<128,blockscale,scatter>") :
                 kOut == 2 ? (kGn128 ? "gemm_fp8_kernel<128,blockscale,split_cat>" : "gemm_fp8_kernel<128,blockscale,gn1,split_cat>") :
                 kOut == 3 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,grouped>" : "gemm_fp8_kernel<128,blockscale,grouped>") :
@@ -1023,6 +1239,48 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
                 kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale>" : kGn128 ? "gemm_fp8_kernel<128,blockscale>" : "gemm_fp8_kernel<128,blockscale,gn1>")
                             : (BN == 256 ? "gemm_fp8_kernel<256,pts>" : BN == 128 ? "gemm_fp8_kernel<128,pts>" : "gemm_fp8_kernel<64,pts>"));
     return check_launch("gemm_fp8_kernel");
+}
+
+// Tile width and CTAs per tile of the kernels with an epilogue of their own (kOut 5, 6).  All tiles take the same time, so what counts
+// is waves x (K blocks per CTA x the time of one, which grows with the share of the SMs at work), at least the time of the epilogue
+// (per-token: it runs beside the next tile's main loop) or plus it (block scales: the accumulators are in its registers); what a wider
+// tile adds once, at the end; and for a split its barriers and exchange and a sixth on every K block.  The weights cannot come faster
+// than 5 TB/s.  The constants are fits of the figures at the two callers below.
+struct TilePlan { int bn, split; };
+struct TileCost { int bn; double lone_us, full_us, least_us, wave_us, once_us, split_us; const void* split_kernel; int threads, smem; };
+template <int kN>
+TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K, int64_t batch, double* us_out = nullptr) {
+    const int64_t sms = sm_count(), kblocks = K / BK;
+    const double stream_us = (double)batch * N * K / 5e6;
+    TilePlan best{0, 1};
+    double best_us = 1e30;
+    for (const TileCost& c : costs) {
+        if (c.bn == 0) continue;
+        const int64_t tiles = (M + BM - 1) / BM * ((N + c.bn - 1) / c.bn) * batch, waves = (tiles + sms - 1) / sms;
+        for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
+            if (split > 1 && (!c.split_kernel || tiles * split > sms || tiles > max_clusters(c.split_kernel, c.threads, c.smem, split))) break;
+            const double busy = tiles * split < sms ? (double)(tiles * split) / sms : 1.0;
+            const double loop = (kblocks + split - 1) / split * (c.lone_us + (c.full_us - c.lone_us) * busy) * (split > 1 ? 1.15 : 1.0);
+            double us = waves * (loop > c.least_us ? loop : c.least_us);
+            us = (us > stream_us ? us : stream_us) + waves * c.wave_us + c.once_us + (split > 1 ? c.split_us + 0.3 * split : 0);
+            if (us < best_us) { best_us = us; best = TilePlan{c.bn, split}; }
+        }
+    }
+    if (us_out) *us_out = best_us;
+    return best;
+}
+
+// Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 8.7 / 9.6 / 9.3,
+// 10.5 / 11.9 / 11.6; x 2048 12.8 / 11.8 / 10.2, 16.2 / 14.8 / 12.9; x 14336 49.0 / 32.4 / 21.9, 70.4 / 42.0 / 28.1; 128 x 1024 x 8192
+// 29.8 / 20.9 / 13.9 (11.0), 40.1 / 26.5 / 18.1 (15.7); 512 x 4096 x 4096 19.9, 25.6 / 21.0; 300 x 14336 x 4096 52.5, 50.1.
+template <int kOut>
+TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool narrow_ok, bool wide_ok) {
+    const TileCost costs[2] = {
+        {narrow_ok ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, (const void*)gemm_fp8_kernel<128, 5, true, true, false, BM, kOut, true>, gemm_threads<128, true>(),
+         SmemLayout<128, 5, false, BM, 128, 32, stage_out_bytes<128, kOut>()>::kDynamic},
+        {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 2, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
+         SmemLayout<256, 3, false, BM, 256, 32, stage_out_bytes<256, kOut>()>::kDynamic}};
+    return plan_tiles(costs, M, N, K, 1);
 }
 
 int common_checks(const char* who, const void* A, const void* B, const void* C, int64_t batch, int64_t M, int64_t N, int64_t K) {
@@ -1052,8 +1310,33 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
                              unsigned long long* trace = nullptr, const Epilogue* ep = nullptr);
 
 namespace {
-// Per-token tiles: `p` complete but for the tile counts.  kOut: 0 plain, 5 with activation and residual.
+// The one-CTA tiles of the per-token scheme: three widths, the narrowest with only the rows of A that exist.
+template <int kOut, bool kSplitK = false>
+int launch_pts_tile(int bn, const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p, cudaStream_t st) {
+    if constexpr (!kSplitK) {
+        if (bn == 256) return launch_gemm<256, 4, false, false, BM, kOut>(tmA, tmB, p, st);
+    }
+    if (bn == 128) return launch_gemm<128, 6, false, false, BM, kOut, kSplitK>(tmA, tmB, p, st);
+    // skinny M with narrow tiles (decode shapes): stage only the A rows that exist, deepen the ring
+    if (p.a_box_rows <= 16) return launch_gemm<64, 19, false, false, 16, kOut, kSplitK>(tmA, tmB, p, st);
+    if (p.a_box_rows <= 64) return launch_gemm<64, 12, false, false, 64, kOut, kSplitK>(tmA, tmB, p, st);
+    return launch_gemm<64, 8, false, false, BM, kOut, kSplitK>(tmA, tmB, p, st);
+}
+
+// CTA pairs: 256 x 256 tiles (a third less operand traffic per SM).
 template <int kOut>
+int launch_pts_pair(const CUtensorMap& tmA, const void* B, GemmParams p, cudaStream_t st) {
+    CUtensorMap tmB, tmBHalf;
+    p.m_blks = (p.M + 255) / 256;
+    p.n_blks = (p.N + 255) / 256;
+    int rc = make_tmap_bytes(&tmB, B, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.batch, 128);
+    if (rc != HKB_OK) return rc;
+    rc = make_tmap_bytes(&tmBHalf, B, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.batch, 64);
+    if (rc != HKB_OK) return rc;
+    return launch_gemm_pair<7, false, kOut>(tmA, tmB, tmBHalf, p, st);
+}
+
+// Per-token tiles, plain; `p` complete but for the tile counts.
 int launch_pts(const void* A, const void* B, GemmParams p, cudaStream_t st) {
     const int64_t M = p.M, N = p.N, K = p.K, batch = p.batch;
     p.m_blks = (int)((M + BM - 1) / BM);
@@ -1071,25 +1354,43 @@ int launch_pts(const void* A, const void* B, GemmParams p, cudaStream_t st) {
     CUtensorMap tmA, tmB;
     int rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, (uint64_t)batch, (uint32_t)p.a_box_rows);
     if (rc != HKB_OK) return rc;
-    // Large problems: CTA pairs on 256 x 256 tiles (a third less operand traffic per SM).
     const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256) * batch;
-    if (bn == 256 && M > 128 && pair_tiles >= sms / 2 && pairs_enabled()) {
-        p.m_blks = (int)((M + 255) / 256);
-        rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, 128);
-        if (rc != HKB_OK) return rc;
-        CUtensorMap tmBHalf;
-        rc = make_tmap_bytes(&tmBHalf, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, 64);
-        if (rc != HKB_OK) return rc;
-        return launch_gemm_pair<7, false, kOut>(tmA, tmB, tmBHalf, p, st);
-    }
+    if (bn == 256 && M > 128 && pair_tiles >= sms / 2 && pairs_enabled()) return launch_pts_pair<0>(tmA, B, p, st);
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, (uint32_t)bn);
     if (rc != HKB_OK) return rc;
-    if (bn == 256) return launch_gemm<256, 4, false, false, BM, kOut>(tmA, tmB, p, st);
-    if (bn == 128) return launch_gemm<128, 6, false, false, BM, kOut>(tmA, tmB, p, st);
-    // skinny M with narrow tiles (decode shapes): stage only the A rows that exist, deepen the ring
-    if (p.a_box_rows <= 16) return launch_gemm<64, 19, false, false, 16, kOut>(tmA, tmB, p, st);
-    if (p.a_box_rows <= 64) return launch_gemm<64, 12, false, false, 64, kOut>(tmA, tmB, p, st);
-    return launch_gemm<64, 8, false, false, BM, kOut>(tmA, tmB, p, st);
+    return launch_pts_tile<0>(bn, tmA, tmB, p, st);
+}
+
+// Per-token tiles with the epilogue; `p` complete but for the tile counts.
+int launch_pts_epilogue(const void* A, const void* B, GemmParams p, cudaStream_t st) {
+    const int64_t M = p.M, N = p.N, K = p.K, batch = p.batch;
+    p.m_blks = (int)((M + BM - 1) / BM);
+    p.a_box_rows = M >= BM ? BM : (int)((M + 7) / 8 * 8);
+    CUtensorMap tmA, tmB;
+    int rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, (uint64_t)batch, (uint32_t)p.a_box_rows);
+    if (rc != HKB_OK) return rc;
+    const void* const narrow = p.a_box_rows <= 16 ? (const void*)gemm_fp8_kernel<64, 19, false, false, false, 16, 5, true>
+                             : p.a_box_rows <= 64 ? (const void*)gemm_fp8_kernel<64, 12, false, false, false, 64, 5, true>
+                                                  : (const void*)gemm_fp8_kernel<64, 8, false, false, false, BM, 5, true>;
+    const int narrow_smem = p.a_box_rows <= 16 ? SmemLayout<64, 19, false, 16>::kDynamic : p.a_box_rows <= 64 ? SmemLayout<64, 12, false, 64>::kDynamic
+                                                                                                            : SmemLayout<64, 8>::kDynamic;
+    const TileCost costs[3] = {{64, 0.18, 0.19, 2, 0, 0, 1.8, narrow, gemm_threads<64, false>(), narrow_smem},
+                               {128, 0.22, 0.255, 3, 0, 1, 2.5, (const void*)gemm_fp8_kernel<128, 6, false, false, false, BM, 5, true>, gemm_threads<128, false>(), SmemLayout<128, 6>::kDynamic},
+                               {256, 0.36, 0.413, 4.5, 0, 2.8, 0, nullptr, 0, 0}};      // not split: behind a narrower tile at every size tried
+    double us = 0;
+    const TilePlan plan = plan_tiles(costs, M, N, K, batch, &us);
+    // CTA pairs take 256 x 256 tiles, the last wave in halves where that is enough (launch_gemm_pair).  64 / 128 / 256-wide tiles / pairs,
+    // us: 512 x 2048 x 1024 5.9 / 7.4 / 10.5 / 11.5, 512 x 4096 x 4096 16.1 / 12.6 / 19.4 / 19.1, 300 x 4096 x 14336 43.5 / 30.3 / 48.7 / 41.4,
+    // 1024 x 14336 x 4096 84.7 / 65.0 / 62.2 / 55.5, 4096 x 4096 x 1024 29.9 / 24.8 / 24.5 / 21.8.  Split, whole / 2 / 4: 128 x 4096 x 14336
+    // 64 wide 24.2 / 19.1 / -; 300 x 1024 x 8192 64 wide 15.0 / 12.4 / -, 128 wide 16.8 / 15.0 / 11.3, 256 wide 25.9 / 20.1 / 15.3.
+    const int64_t pairs = sm_count() / 2, tiles = (M + 255) / 256 * ((N + 255) / 256) * batch, last = tiles % pairs;
+    const double pair_us = (tiles / pairs + (last == 0 ? 0 : tiles > pairs && 2 * last <= pairs ? 0.5 : 1)) * (K / BK * 0.42 > 5 ? K / BK * 0.42 : 5) + 3.8;
+    if (M > 128 && pair_us < us && pairs_enabled()) return launch_pts_pair<5>(tmA, B, p, st);
+    p.split = plan.split;
+    p.n_blks = (int)((N + plan.bn - 1) / plan.bn);
+    rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)N, (uint64_t)batch, (uint32_t)plan.bn);
+    if (rc != HKB_OK) return rc;
+    return plan.split > 1 ? launch_pts_tile<5, true>(plan.bn, tmA, tmB, p, st) : launch_pts_tile<5>(plan.bn, tmA, tmB, p, st);
 }
 }  // namespace
 
@@ -1115,11 +1416,9 @@ int gemm_fp8_pts_impl(const void* A, const void* B, void* C, const float* sa, co
     // Decode shapes: HBM-bound on the weight stream; a kernel that deals the columns out evenly
     // over the SMs (gemm_fp8_skinny.cu).  HKB_GEMM_SKINNY=0 keeps the fixed-width tiles below.
     if (M <= 64 && batch == 1 && N % 16 == 0 && aligned32(C) && skip_kblock < 0 && skinny_enabled()) {
-        note_kernel(ep ? "gemm_fp8_skinny_kernel<epilogue>" : "gemm_fp8_skinny_kernel");
         return launch_gemm_fp8_skinny(A, B, C, sa, sb, bias, ep ? &ep->act : nullptr, ep ? ep->residual : nullptr, M, N, K, p.status, (cudaStream_t)stream);
     }
-    if (ep) return launch_pts<5>(A, B, p, (cudaStream_t)stream);
-    return launch_pts<0>(A, B, p, (cudaStream_t)stream);
+    return ep ? launch_pts_epilogue(A, B, p, (cudaStream_t)stream) : launch_pts(A, B, p, (cudaStream_t)stream);
 }
 }  // namespace hkb
 
@@ -1297,7 +1596,6 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     // Decode shapes: the weight stream bounds them (gemm_fp8_blockscale_skinny.cu).  At 32 tokens it is
     // ahead for every N and K tried, at 64 behind (figures there).
     if (M <= 32 && gn == 128 && !sc && n_peer == 0 && !trace) {
-        note_kernel(ep ? "gemm_fp8_blockscale_skinny_kernel<epilogue>" : "gemm_fp8_blockscale_skinny_kernel");
         BsSkinnyOut out{C, ldc};
         out.c_a = c_a;
         out.c_b = c_b;
@@ -1309,6 +1607,11 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     const int sms = sm_count();
     int bn = 256;
     if (gn != 128 || sc || N % 256 != 0 || (int64_t)p.m_blks * (N / 256) < 2LL * sms) bn = 128;
+    if (ep && gn == 128) {
+        const TilePlan plan = plan_block_scale<5>(M, N, K, true, N % 256 == 0);
+        bn = plan.bn;
+        p.split = plan.split;
+    }
     p.n_blks = (int)(N / bn);
     cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap tmA, tmB;
@@ -1345,6 +1648,7 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     }
     if (ep) {
         if (gn != 128) return launch_gemm<128, 6, true, false, BM, 5>(tmA, tmB, p, st);
+        if (p.split > 1) return bn == 256 ? launch_gemm<256, 3, true, true, BM, 5, true>(tmA, tmB, p, st) : launch_gemm<128, 5, true, true, BM, 5, true>(tmA, tmB, p, st);
         if (bn == 256) return launch_gemm<256, 3, true, true, BM, 5>(tmA, tmB, p, st);
         return launch_gemm<128, 5, true, true, BM, 5>(tmA, tmB, p, st);
     }
@@ -1393,7 +1697,6 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     rc = status_word(&status);
     if (rc != HKB_OK) return rc;
     if (M <= kGatedDecodeRows) {
-        note_kernel("gemm_fp8_blockscale_skinny_kernel<gated>");
         BsSkinnyOut out{C, F};
         out.gated = true;
         out.act = act;
@@ -1410,15 +1713,16 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     p.wait_ns = kWaitLimitNs; p.skip_kblock = -1; p.status = status;
     p.m_blks = (int)((M + BM - 1) / BM);
     p.a_box_rows = BM;
-    // 128 output columns per tile where that gives every SM two tiles, as in the plain GEMM, and for FP8 output always: a tile has
-    // to hold whole scale groups
-    const int bn = c_scale || p.m_blks * (F / 128) >= 2LL * sm_count() ? 256 : 128;
+    const TilePlan plan = plan_block_scale<6>(M, 2 * F, K, c_scale == nullptr, true);        // FP8: a tile has to hold whole scale groups
+    const int bn = plan.bn;
+    p.split = plan.split;
     p.n_blks = (int)(F / (bn / 2));
     CUtensorMap tmA, tmB;
     rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, 1, BM);
     if (rc != HKB_OK) return rc;
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)(2 * F), 1, (uint32_t)bn / 2);
     if (rc != HKB_OK) return rc;
+    if (p.split > 1) return bn == 256 ? launch_gemm<256, 3, true, true, BM, 6, true>(tmA, tmB, p, st) : launch_gemm<128, 5, true, true, BM, 6, true>(tmA, tmB, p, st);
     if (bn == 256) return launch_gemm<256, 3, true, true, BM, 6>(tmA, tmB, p, st);
     return launch_gemm<128, 5, true, true, BM, 6>(tmA, tmB, p, st);
 }

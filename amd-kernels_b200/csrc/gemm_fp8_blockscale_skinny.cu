@@ -27,6 +27,11 @@
 // Gated (kOut == 2): a tile is up to 64 output columns, its MMA rows the gate rows of those columns and behind them the up rows (two
 // boxes).  Behind the last K block the threads of the up rows hand their sums to those of the gate rows through shared memory.
 //
+// Split K (kSplitK, kOut 1 and 2): one tile of a narrow layer is a long chain of K steps on a few SMs.  There a cluster of 2, 4 or 8 CTAs
+// shares a tile, each with a part of K; at the end all write their sums into the first one's (by then idle) operand ring through
+// distributed shared memory and it adds them in rank order, so the result is the same every time.  The two cluster barriers around
+// that are reached by every thread on every path, an abandoned wait included.  plan_split() below has the rule.
+//
 // Roles: warp 0 TMA producer, warp 1 TMEM allocator + MMA issuer, warps 2-9 epilogue, warps 10-11 scale staging.  Bounded
 // waits and teardown as in gemm_fp8.cu.
 #include "activation.cuh"
@@ -56,6 +61,7 @@ struct BsSkinnyParams {
     int M, N, K;
     int64_t ldc;
     int a_box_rows;                       // rows of A fetched per stage (multiple of 8, <= 32)
+    int split;                            // CTAs per tile (cluster size); above 1 every cluster has exactly one tile
     int tiles, base, rem;                 // tile t is base + (t < rem) units high and starts at unit t*base + min(t, rem)
     int stages, sub_bytes, a_off;         // one K block inside a stage; its activation rows
     const float* sa;
@@ -79,7 +85,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
 #define TILE_ROW0(t) (((t) * p.base + min((t), p.rem)) * 16)
 
 // NT: token columns (16 or 32).  kOut: 0 plain / multiply-add, 1 bias + activation + residual, 2 gated (p.N output columns, B has 2N rows).
-template <int NT, int kOut>
+template <int NT, int kOut, bool kSplitK = false>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                                   const __grid_constant__ CUtensorMap tmB1, const BsSkinnyParams p) {
@@ -105,8 +111,16 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int kblocks = p.K / 128;
-    const int ksteps = (kblocks + kStep - 1) / kStep;       // an odd last block is followed by zero-filled data and zero scales
+    const int all_kblocks = p.K / 128;
+    const int all_ksteps = (all_kblocks + kStep - 1) / kStep;       // an odd last block is followed by zero-filled data and zero scales
+    const int split = kSplitK ? p.split : 1;
+    const int rank = kSplitK ? (int)cluster_ctarank() : 0;
+    const int ks0 = all_ksteps * rank / split;                      // this CTA's part of K: whole steps, the odd block stays last
+    const int ksteps = all_ksteps * (rank + 1) / split - ks0;
+    const int kblock0 = ks0 * kStep;
+    const int kblocks = min(ksteps * kStep, all_kblocks - kblock0);
+    const int tile0 = kSplitK ? (int)blockIdx.x / split : (int)blockIdx.x;
+    const int tile_step = kSplitK ? (int)gridDim.x / split : (int)gridDim.x;
     const uint32_t stage_bytes = kStep * p.sub_bytes;
     const int nchunks = (kblocks + kChunk - 1) / kChunk;
 
@@ -142,7 +156,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
             int s = 0;
             uint32_t ph = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+            for (int t = tile0; t < p.tiles && ok; t += tile_step) {
                 const CUtensorMap* const tmB = t < p.rem ? &tmB1 : &tmB0;
                 const int n0 = TILE_ROW0(t);
                 const uint32_t b_bytes = (uint32_t)TILE_UNITS(t) * 2048;
@@ -153,9 +167,9 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
                     const uint32_t st = ring_base + s * stage_bytes;
 #pragma unroll
                     for (int i = 0; i < kStep; ++i) {
-                        tma_load_3d(st + i * p.sub_bytes, tmB, full_bar(s), (ks * kStep + i) * 128, n0, 0);
-                        if constexpr (kGated) tma_load_3d(st + i * p.sub_bytes + b_bytes, tmB, full_bar(s), (ks * kStep + i) * 128, p.N + n0, 0);
-                        tma_load_3d(st + i * p.sub_bytes + p.a_off, &tmA, full_bar(s), (ks * kStep + i) * 128, 0, 0);
+                        tma_load_3d(st + i * p.sub_bytes, tmB, full_bar(s), (kblock0 + ks * kStep + i) * 128, n0, 0);
+                        if constexpr (kGated) tma_load_3d(st + i * p.sub_bytes + b_bytes, tmB, full_bar(s), (kblock0 + ks * kStep + i) * 128, p.N + n0, 0);
+                        tma_load_3d(st + i * p.sub_bytes + p.a_off, &tmA, full_bar(s), (kblock0 + ks * kStep + i) * 128, 0, 0);
                     }
                     if (++s == p.stages) { s = 0; ph ^= 1; }
                 }
@@ -169,7 +183,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
             int acc = 0;
             uint32_t acc_ph = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+            for (int t = tile0; t < p.tiles && ok; t += tile_step) {
                 for (int ks = 0; ks < ksteps; ++ks) {
                     if (!mbar_wait(full_bar(s), ph, abort_flag, p.status, kErrWaitMma)) { ok = false; break; }
                     if (!mbar_wait(tempty_bar(acc), acc_ph ^ 1, abort_flag, p.status, kErrWaitMma)) { ok = false; break; }
@@ -199,7 +213,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
         int acc = 0, slot = 0, s = 0;
         uint32_t acc_ph = 0, slot_ph = 0, x_ph = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+        for (int t = tile0; t < p.tiles && ok; t += tile_step) {
             const int cols = TILE_UNITS(t) * 16;                         // output columns of the tile
             const int rows = kGated ? 2 * cols : cols;
             const int n0 = TILE_ROW0(t);
@@ -269,6 +283,31 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
                 if (lane == 0) mbar_arrive(sempty_bar(slot));
                 if (++slot == kSlots) { slot = 0; slot_ph ^= 1; }
             }
+            if constexpr (kSplitK) {
+                {
+                    __syncwarp();
+                    cluster_sync_all();                    // every CTA of the cluster is done with its operand ring
+                    const uint32_t slot0 = ring_base + (uint32_t)(col0 * 128 + row_in_tile) * 4;        // [rank - 1][token][row]
+                    if (ok && rank != 0 && warp_has_rows) {
+                        const uint32_t dst = cluster_addr(slot0 + (uint32_t)(rank - 1) * (NT * 512), 0);
+#pragma unroll
+                        for (int j = 0; j < NC; ++j) st_cluster(dst + j * 512, (j & 1) ? acc2[j / 2].y : acc2[j / 2].x);
+                    }
+                    __syncwarp();
+                    cluster_sync_all();
+                    if (rank != 0) break;                  // the only tile of this cluster
+                    if (warp_has_rows) {
+                        const float* const part = reinterpret_cast<const float*>(smem + (slot0 - bar_base));
+                        for (int r = 0; r < split - 1; ++r) {
+#pragma unroll
+                            for (int j = 0; j < NC; ++j) {
+                                const float v = part[(r * NT + j) * 128];
+                                if (j & 1) acc2[j / 2].y += v; else acc2[j / 2].x += v;
+                            }
+                        }
+                    }
+                }
+            }
             if constexpr (kGated) {
                 // the up sums change hands: written, all eight warps arrive, read by the gate rows, all arrive before the next tile writes
                 float* const xr = xchg + col0 * kXchgPitch + (n - n0);
@@ -336,20 +375,20 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
         // ================= scale staging: warp g fills every second slot =================
         const int g = warp - 2 - kEpiWarps;
         const int nsb = p.N / 128;                           // gated: of gate and of up
-        const bool vec = (kblocks & 3) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
+        const bool vec = (all_kblocks & 3) == 0 && (kblock0 & 3) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
         int slot = g, ch = g;                                // ch: chunk of the tile, in the epilogue's order
         uint32_t ph = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+        for (int t = tile0; t < p.tiles && ok; t += tile_step) {
             const int g0 = TILE_ROW0(t) >> 7;
             for (; ch < nchunks; ch += 2) {
                 const int kb0 = ch * kChunk;
                 const int kn = min(kblocks - kb0, kChunk);
                 float v[kChunk];
-                const float* const src = p.sa + (int64_t)lane * kblocks + kb0;
+                const float* const src = p.sa + (int64_t)lane * all_kblocks + kblock0 + kb0;
 #pragma unroll
                 for (int k = 0; k < kChunk; k += 4) {
-                    if (lane < p.M && vec && k < kn) {       // kblocks % 4 == 0: whole vectors
+                    if (lane < p.M && vec && k + 4 <= kn) {
                         const float4 f = __ldg(reinterpret_cast<const float4*>(src + k));
                         v[k] = f.x; v[k + 1] = f.y; v[k + 2] = f.z; v[k + 3] = f.w;
                     } else {
@@ -360,7 +399,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
                 // two weight scales per K block (gated: two of gate, two of up)
                 constexpr int W = kGated ? 4 : 2;
                 const int wk = lane / W, wi = lane % W, wg = min(g0 + (wi & 1), nsb - 1) + (wi >> 1) * nsb;
-                const float wsc = wk < kn ? __ldg(p.sb + (int64_t)(kb0 + wk) * (W / 2 * nsb) + wg) : 0.0f;
+                const float wsc = wk < kn ? __ldg(p.sb + (int64_t)(kblock0 + kb0 + wk) * (W / 2 * nsb) + wg) : 0.0f;
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(sempty_bar(slot), ph ^ 1, abort_flag, p.status, kErrWaitProducer))) { ok = false; break; }
                 float* const dst = scales + slot * kChunk * kPitch;
 #pragma unroll
@@ -375,6 +414,13 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
         }
     }
 
+    if constexpr (kSplitK) {
+        if ((warp < 2 || warp >= 2 + kEpiWarps)) {            // the epilogue warps' two cluster barriers, reached by everyone
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -390,21 +436,52 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
 #undef TILE_UNITS
 #undef TILE_ROW0
 
-template <int NT, int kOut>
+template <int NT, int kOut, bool kSplitK = false>
 int launch(const CUtensorMap& tmA, const CUtensorMap& tmB0, const CUtensorMap& tmB1, const BsSkinnyParams& p, int smem, int grid, cudaStream_t st) {
     // the limit is the kernel's, not the call's: every call sets the same one, whatever its own size (calls may overlap)
-    auto kern = gemm_fp8_blockscale_skinny_kernel<NT, kOut>;
+    auto kern = gemm_fp8_blockscale_skinny_kernel<NT, kOut, kSplitK>;
     HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
-    HKB_CUDA(launch_dependent(true, kern, grid, kThreads, smem, 0, st, tmA, tmB0, tmB1, p));
+    note_kernel(kOut == 0 ? "gemm_fp8_blockscale_skinny_kernel" :
+                kOut == 1 ? (kSplitK ? "gemm_fp8_blockscale_skinny_kernel<epilogue,split>" : "gemm_fp8_blockscale_skinny_kernel<epilogue>")
+                          : (kSplitK ? "gemm_fp8_blockscale_skinny_kernel<gated,split>" : "gemm_fp8_blockscale_skinny_kernel<gated>"));
+    HKB_CUDA(launch_dependent(true, kern, grid, kThreads, smem, kSplitK ? p.split : 0, st, tmA, tmB0, tmB1, p));
     return check_launch("gemm_fp8_blockscale_skinny_kernel");
 }
 
 template <int NT>
 int launch_out(const CUtensorMap& tmA, const CUtensorMap& tmB0, const CUtensorMap& tmB1, const BsSkinnyParams& p, const BsSkinnyOut& out, int smem,
                int grid, cudaStream_t st) {
+    if (p.split > 1) return out.gated ? launch<NT, 2, true>(tmA, tmB0, tmB1, p, smem, grid, st) : launch<NT, 1, true>(tmA, tmB0, tmB1, p, smem, grid, st);
     if (out.gated) return launch<NT, 2>(tmA, tmB0, tmB1, p, smem, grid, st);
     if (out.epilogue) return launch<NT, 1>(tmA, tmB0, tmB1, p, smem, grid, st);
     return launch<NT, 0>(tmA, tmB0, tmB1, p, smem, grid, st);
+}
+
+// How many CTAs share a tile.  A K step (two blocks) takes about 0.32 us (0.41 with 32 token columns) on the MMA thread and its
+// hand-off and 8 ns more per KB of weights, or the time in which an SM pulls them (45 bytes per ns when all SMs do); a split adds
+// about 2 us: the clusters' barriers and the partial sums.  The split that this puts ahead is taken, if all its clusters fit the device at once.
+// 16 tokens, us, whole / 2 / 4 / 8 CTAs per tile: N = 1024, K = 1024 4.9 / 5.4 / 5.1 / 4.9, K = 4096 9.2 / 7.7 / 6.4 / 6.4, K = 14336
+// 23.9 / 15.8 / 10.3 / 8.3; N = 4096, K = 1024 5.0 / 5.5 / 5.7 / -, K = 4096 9.5 / 7.8 / 7.1 / -, K = 14336 25.4 / 18.0 / 15.1 / -.
+void plan_split(bool nt16, const BsSkinnyOut& out, int64_t units, int parts, int ksteps, int64_t rounds, BsSkinnyParams& p) {
+    const void* const kern = nt16 ? (out.gated ? (const void*)gemm_fp8_blockscale_skinny_kernel<16, 2, true> : (const void*)gemm_fp8_blockscale_skinny_kernel<16, 1, true>)
+                                  : (out.gated ? (const void*)gemm_fp8_blockscale_skinny_kernel<32, 2, true> : (const void*)gemm_fp8_blockscale_skinny_kernel<32, 1, true>);
+    auto step_us = [&](int64_t height) {
+        const double kb = 4.0 * height * parts, pull = kb / 44, hand_off = (nt16 ? 0.32 : 0.41) + 0.008 * kb;
+        return pull > hand_off ? pull : hand_off;
+    };
+    double best = rounds * ksteps * step_us((units + p.tiles - 1) / p.tiles);
+    for (int split = 2; split <= 8 && split <= ksteps; split *= 2) {
+        const int64_t clusters = max_clusters(kern, kThreads, kSmemLimit, split);
+        if (clusters == 0) break;
+        const int64_t tiles = units < clusters ? units : clusters, height = (units + tiles - 1) / tiles;
+        if (height * parts > kMaxUnits) break;
+        const double us = (ksteps + split - 1) / split * step_us(height) + 2;
+        if (us < best) {
+            best = us;
+            p.split = split;
+            p.tiles = (int)tiles;
+        }
+    }
 }
 
 }  // namespace
@@ -424,7 +501,9 @@ int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, const float*
     const int parts = out.gated ? 2 : 1;                  // gate and up rows share the 128 MMA rows
     const int max_units = kMaxUnits / parts;
     const int64_t rounds = (units + (int64_t)max_units * sms - 1) / ((int64_t)max_units * sms);
+    p.split = 1;
     p.tiles = (int)(units < rounds * sms ? units : rounds * sms);
+    if (out.gated || out.epilogue) plan_split(nt == 16, out, units, parts, (int)((K / 128 + kStep - 1) / kStep), rounds, p);
     p.base = (int)(units / p.tiles);
     p.rem = (int)(units % p.tiles);
     const int maxu = p.base + (p.rem ? 1 : 0);
@@ -442,7 +521,7 @@ int launch_gemm_fp8_blockscale_skinny(const void* A, const void* B, const float*
     if (rc != HKB_OK) return rc;
     rc = make_tmap_bytes(&tmB1, B, (uint64_t)K, (uint64_t)(parts * N), 1, (uint32_t)maxu * 16);
     if (rc != HKB_OK) return rc;
-    const int grid = p.tiles < sms ? p.tiles : sms;
+    const int grid = p.split > 1 ? p.tiles * p.split : p.tiles < sms ? p.tiles : sms;
     if (nt == 16) return launch_out<16>(tmA, tmB0, tmB1, p, out, smem, grid, st);
     return launch_out<32>(tmA, tmB0, tmB1, p, out, smem, grid, st);
 }

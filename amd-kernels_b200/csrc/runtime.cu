@@ -55,6 +55,33 @@ int sm_count() {
     return g_dev[dev].sms;
 }
 
+int max_clusters(const void* kern, int threads, int smem, int cluster) {
+    struct Entry { int dev; const void* kern; int cluster, n; };
+    static Entry table[64];
+    static int used = 0;
+    int dev = 0;
+    if (current_device(&dev) != HKB_OK) return 0;
+    std::lock_guard<std::mutex> lk(g_mu);
+    for (int i = 0; i < used; ++i)
+        if (table[i].dev == dev && table[i].kern == kern && table[i].cluster == cluster) return table[i].n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (!cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) ||
+        !cuda_ok(cudaOccupancyMaxActiveClusters(&n, kern, &cfg)))
+        n = 0;
+    if (used < (int)(sizeof table / sizeof table[0])) table[used++] = Entry{dev, kern, cluster, n};
+    return n;
+}
+
 int scratch_get(ScratchSlot slot, cudaStream_t stream, size_t bytes, void** out) {
     int dev = 0;
     int rc = current_device(&dev);

@@ -264,6 +264,16 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_dst, uint32_t ncol
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {    // one warp in EACH CTA
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
+// Address of this CTA's shared-memory location in CTA `cta` of the cluster, and plain stores there.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t smem, uint32_t cta) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(cta));
+    return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
 // Arrive (once all earlier tcgen05 ops of this thread are done) on the barrier at this offset in
 // every CTA of `mask`.
 __device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t mask) {

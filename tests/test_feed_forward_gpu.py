@@ -222,21 +222,32 @@ def test_linear_optional_operands(hk, scales, M, bias, residual):
     check_linear(hk, scales, 1, M, 256, 384, bias=bias, residual=residual, act="silu")
 
 
+PTS = "gemm_fp8_kernel<{},pts,epilogue{}>".format
+BLOCK = "gemm_fp8_kernel<{},blockscale,epilogue{}>".format
+
+
 @pytest.mark.parametrize("batch,M,N,K,kernel", [
     (1, 1, 1024, 128, "gemm_fp8_skinny_kernel<epilogue>"), (1, 64, 2064, 1024, "gemm_fp8_skinny_kernel<epilogue>"),
-    (1, 16, 1032, 256, "gemm_fp8_kernel<64,pts,epilogue>"), (1, 61, 8, 256, "gemm_fp8_kernel<64,pts,epilogue>"),
-    (3, 77, 1032, 384, "gemm_fp8_kernel<64,pts,epilogue>"), (2, 13, 520, 256, "gemm_fp8_kernel<64,pts,epilogue>"),
-    (1, 1000, 9000, 256, "gemm_fp8_kernel<128,pts,epilogue>"), (1, 127, 80000, 128, "gemm_fp8_kernel<256,pts,epilogue>"),
-    (1, 2049, 9480, 256, "gemm_fp8_kernel<256,pts,pair,epilogue>"), (8, 512, 4096, 256, "gemm_fp8_kernel<256,pts,pair,epilogue>")])
+    (1, 5, 1024, 8192, "gemm_fp8_skinny_kernel<epilogue,split>"), (1, 64, 1040, 4224, "gemm_fp8_skinny_kernel<epilogue,split>"),
+    (1, 33, 4096, 14336, "gemm_fp8_skinny_kernel<epilogue,split>"),
+    (1, 16, 1032, 256, PTS(64, "")), (1, 61, 8, 256, PTS(64, "")), (3, 77, 1032, 384, PTS(64, "")), (2, 13, 520, 256, PTS(64, "")),
+    (1, 16, 1032, 4096, PTS(64, ",split")), (1, 61, 1032, 4224, PTS(64, ",split")), (2, 40, 520, 4096, PTS(64, ",split")), (1, 300, 504, 8192, PTS(64, ",split")),
+    (1, 127, 80000, 128, PTS(128, "")), (1, 2048, 1024, 8192, PTS(128, "")),
+    (1, 300, 1024, 8192, PTS(128, ",split")), (1, 170, 1272, 9728, PTS(128, ",split")),
+    (1, 1000, 9000, 256, PTS(256, "")), (1, 2049, 9480, 256, PTS(256, "")), (4, 302, 640, 13824, PTS(128, ",split")),
+    (1, 4000, 4040, 2048, PTS("256", "").replace("pts", "pts,pair")), (2, 134, 9584, 4736, PTS("256", "").replace("pts", "pts,pair"))])
 def test_linear_per_token_kernels(hk, batch, M, N, K, kernel):
     check_linear(hk, "token", batch, M, N, K, act="gelu_tanh", kernel=kernel)
 
 
 @pytest.mark.parametrize("M,N,K,gn,kernel", [
     (1, 128, 128, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue>"), (32, 1152, 896, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue>"),
-    (17, 28672, 256, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue>"), (33, 1152, 384, 128, "gemm_fp8_kernel<128,blockscale,epilogue>"),
-    (300, 128, 5248, 128, "gemm_fp8_kernel<128,blockscale,epilogue>"), (1025, 9728, 256, 128, "gemm_fp8_kernel<256,blockscale,epilogue>"),
-    (200, 256, 384, 1, "gemm_fp8_kernel<128,blockscale,gn1,epilogue>"), (3, 128, 128, 1, "gemm_fp8_kernel<128,blockscale,gn1,epilogue>")])
+    (17, 28672, 256, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue>"), (32, 1024, 8192, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue,split>"),
+    (9, 2048, 4224, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue,split>"), (3, 4096, 14336, 128, "gemm_fp8_blockscale_skinny_kernel<epilogue,split>"),
+    (33, 1152, 384, 128, BLOCK(128, "")), (1025, 9728, 256, 128, BLOCK(128, "")),
+    (300, 128, 5248, 128, BLOCK(128, ",split")), (40, 128, 8320, 128, BLOCK(128, ",split")),
+    (1025, 9728, 1024, 128, BLOCK(256, "")), (300, 4096, 14336, 128, BLOCK(256, ",split")), (600, 1024, 8320, 128, BLOCK(256, ",split")),
+    (200, 256, 384, 1, BLOCK(128, "").replace("scale", "scale,gn1")), (3, 128, 128, 1, BLOCK(128, "").replace("scale", "scale,gn1"))])
 def test_linear_block_scale_kernels(hk, M, N, K, gn, kernel):
     check_linear(hk, "block", 1, M, N, K, act="gelu", gn=gn, kernel=kernel)
 
@@ -344,20 +355,23 @@ def test_gated_activations(hk, M, act, fp8):
     check_gated(hk, M, 256, 256, act, fp8)
 
 
-SKINNY, WIDE, NARROW = "gemm_fp8_blockscale_skinny_kernel<gated>", "gemm_fp8_kernel<256,blockscale,gated>", "gemm_fp8_kernel<128,blockscale,gated>"
+DECODE = "gemm_fp8_blockscale_skinny_kernel<gated{}>".format
+GATED = "gemm_fp8_kernel<{},blockscale,gated{}>".format
 
 
 @pytest.mark.parametrize("M,F,K,fp8,kernel", [
-    (1, 128, 128, False, SKINNY), (1, 128, 128, True, SKINNY), (16, 14336, 256, True, SKINNY), (17, 1152, 1152, False, SKINNY), (32, 28672, 384, True, SKINNY),
-    (32, 640, 2176, False, SKINNY), (33, 128, 128, True, WIDE), (33, 128, 128, False, NARROW), (300, 1152, 4224, True, WIDE), (257, 640, 384, False, NARROW),
-    (1025, 9600, 256, False, WIDE), (1300, 4096, 128, True, WIDE)])
+    (1, 128, 128, False, DECODE("")), (1, 128, 128, True, DECODE("")), (16, 14336, 256, True, DECODE("")), (17, 1152, 1152, False, DECODE("")),
+    (32, 28672, 384, True, DECODE("")), (32, 640, 2176, False, DECODE(",split")), (9, 1024, 4224, True, DECODE(",split")), (31, 128, 8192, True, DECODE(",split")),
+    (33, 128, 128, True, GATED(256, "")), (33, 128, 128, False, GATED(128, "")), (257, 640, 384, False, GATED(128, "")),
+    (200, 640, 4224, False, GATED(128, ",split")), (130, 1024, 8192, False, GATED(128, ",split")), (40, 128, 8320, False, GATED(128, ",split")),
+    (300, 1152, 4224, True, GATED(256, ",split")), (70, 256, 2048, True, GATED(256, ",split")), (40, 128, 8320, True, GATED(256, ",split")),
+    (1025, 9600, 256, False, GATED(256, "")), (1300, 4096, 128, True, GATED(256, ""))])
 def test_gated_kernels(hk, M, F, K, fp8, kernel):
     check_gated(hk, M, F, K, "silu", fp8, kernel)
 
 
 def test_gated_zero_infinite_and_nan_rows(hk):
-    for M in (6, 70):
-        F, K = 256, 256
+    for M, F, K in ((6, 256, 256), (70, 256, 256), (6, 256, 4096), (70, 256, 4096)):
         a, b, sa, sb, *_ = gated_case(M, F, K, 9)
         sa[0] = 0
         sa[1] = float("nan")
@@ -412,7 +426,7 @@ def test_gated_layer(hk, M, D, F):
 
 
 def test_layers_captured_replayed_and_on_two_streams(hk):
-    shapes = [(24, 1024, 2048), (200, 512, 1152)]
+    shapes = [(24, 1024, 2048), (200, 512, 1152), (150, 512, 8192), (8, 512, 8192)]
     for M, D, F in shapes:
         eager, graphed, other = (GatedLayer(M, D, F, 1) for _ in range(3))
         start = eager.h.clone()
