@@ -17,7 +17,8 @@ namespace {
 
 constexpr float kFp8Max = 448.0f;
 constexpr float kScaleFloor = 1e-10f;
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;          // of the flat kernel, and of a CTA of several teams
+constexpr int kMaxWarps = 16;          // of a team
 
 // EL bf16 (8 or 16) of one row.  Plain loads, not the read-only path: residual_out may be x or residual.
 template <int EL> struct Chunk { uint32_t w[EL / 2]; };
@@ -44,33 +45,32 @@ struct AddNormParams {
     int64_t M;
     int D;
     float eps;
+    int warps;             // of a team
 };
 
-// TPR threads share a row (256 / TPR rows per CTA), a thread holds NW chunks of EL elements, chunk index t + i * TPR.  The 128
-// columns of a scale group lie in 128 / EL neighbouring lanes of one i.  Rows of a CTA meet on their own named barrier only.
-template <int EL, int NW, int TPR, bool kRowScale>
-__global__ void __launch_bounds__(kThreads)
+// A team of `warps` warps has a row (blockDim / team rows per CTA), a thread holds NW chunks of EL elements, chunk index t + i * team.
+// The 128 columns of a scale group lie in 128 / EL neighbouring lanes of one i.  Teams of a CTA meet on their own named barrier only.
+template <int EL, int NW, bool kRowScale>
+__global__ void __launch_bounds__(32 * kMaxWarps)
 add_rmsnorm_quant_kernel(const AddNormParams p) {
     pdl_trigger();
     pdl_wait();
-    constexpr int RPB = kThreads / TPR, WPR = TPR / 32;
-    const int tid = threadIdx.x, r_in = tid / TPR, t = tid % TPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + r_in;
+    const int team = 32 * p.warps, r_in = (int)threadIdx.x / team, t = (int)threadIdx.x - r_in * team;
+    const int64_t row = (int64_t)blockIdx.x * ((int)blockDim.x / team) + r_in;
     const bool live = row < p.M;
     const int chunks = p.D / EL;
     const int64_t base = row * p.D;
 
-    __shared__ float s_part[2][kThreads / 32];
+    __shared__ float s_part[2][kMaxWarps];
     auto row_reduce = [&](int which, float v, auto op) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-        if constexpr (WPR > 1) {
-            if ((tid & 31) == 0) s_part[which][tid >> 5] = v;
-            if constexpr (TPR == kThreads) __syncthreads();
-            else asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "r"(TPR) : "memory");
-            v = s_part[which][r_in * WPR];
-#pragma unroll
-            for (int k = 1; k < WPR; ++k) v = op(v, s_part[which][r_in * WPR + k]);
+        if (p.warps > 1) {
+            float* const part = s_part[which] + r_in * p.warps;
+            if ((t & 31) == 0) part[t >> 5] = v;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "r"(team) : "memory");
+            v = part[0];
+            for (int k = 1; k < p.warps; ++k) v = op(v, part[k]);
         }
         return v;
     };
@@ -80,7 +80,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
         Chunk<EL> a[NW];
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            const int c = t + i * TPR;
+            const int c = t + i * team;
             if (live && c < chunks) {
                 load(a[i], p.x + base + (int64_t)c * EL);
                 load(h[i], p.residual + base + (int64_t)c * EL);
@@ -101,7 +101,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
     float2 ss2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-        const int c = t + i * TPR;
+        const int c = t + i * team;
         if (live && c < chunks) store(p.sum + base + (int64_t)c * EL, h[i]);
 #pragma unroll
         for (int j = 0; j < EL / 2; ++j) { const float2 f = bf16x2_to_f2(h[i].w[j]); ss2 = __ffma2_rn(f, f, ss2); }
@@ -112,7 +112,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
 
     // y of chunk i, computed where it is needed: the gain comes from L1 / L2
     auto normed = [&](int i, float2 (&y)[EL / 2]) {
-        const int c = t + i * TPR;
+        const int c = t + i * team;
         uint4 w[EL / 8];
 #pragma unroll
         for (int k = 0; k < EL / 8; ++k)
@@ -128,7 +128,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
     };
     // y is defined up to the order of the sum of squares, so the quotient is y * RN(1/scale), within one fp32 ulp of the division.
     auto emit = [&](int i, const float2 (&y)[EL / 2], float rs) {
-        const int c = t + i * TPR;
+        const int c = t + i * team;
         const float2 rs2 = make_float2(rs, rs);
         uint32_t o[EL / 4];
 #pragma unroll
@@ -162,41 +162,38 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
             for (int o = LANES / 2; o > 0; o >>= 1) am = max_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
             const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor);
             emit(i, y, __frcp_rn(scale));
-            const int c = t + i * TPR;
+            const int c = t + i * team;
             if (live && c < chunks && t % LANES == 0) sr[c / LANES] = scale;
         }
     }
 }
 
-template <int EL, int NW, bool kRowScale>
-int launch_add_norm(int tpr, const AddNormParams& p, cudaStream_t st) {
-    const unsigned grid = (unsigned)((p.M + kThreads / tpr - 1) / (kThreads / tpr));
-    auto kern = add_rmsnorm_quant_kernel<EL, NW, 256, kRowScale>;
-    if constexpr (EL * NW <= 64) {           // narrower teams hold at most 64 elements per thread
-        if (tpr == 32) kern = add_rmsnorm_quant_kernel<EL, NW, 32, kRowScale>;
-        if (tpr == 64) kern = add_rmsnorm_quant_kernel<EL, NW, 64, kRowScale>;
-        if (tpr == 128) kern = add_rmsnorm_quant_kernel<EL, NW, 128, kRowScale>;
-    }
-    HKB_CUDA(launch_dependent(true, kern, grid, kThreads, 0, 0, st, p));
-    return check_launch("add_rmsnorm_quant_kernel");
-}
-
+// Chunks per thread.  Few rows, where only latency counts: one, as many warps per row as it takes.  Else 32 elements per thread (24 in
+// 8-element chunks) in teams of up to 16 (8) warps, more only for rows that need it.  us with 1 / 2 / 3 / 4 chunks of 16: 300 x 4096
+// 3.3 / 4.0 / 4.0 / 4.3, 1000 x 5120 8.0 / 8.3 / 9.3 / 9.6, 4096 x 4096 22.5 / 20.8 / 22.4 / 22.2, 4096 x 5120 31.7 / 26.9 / 27.2 / 31.7,
+// 16384 x 8192 144 / 138 / 149 / 141 (only 1000 x 4096 differs: 6.7 / 6.7 / 6.1 / 5.8); with 1 / 2 / 3 / 4 / 6 / 8 chunks of 8: 8000 x 1032
+// 29.7 / 20.3 / 14.3 / 16.2 / 15.0 / 15.2, 8000 x 2056 35.2 / 34.6 / 25.4 / 25.6 / 29.1 / 29.0, 4000 x 16376 - / - / - / 106 / 114 / 77.
 template <int EL, bool kRowScale>
-int dispatch_add_norm(const AddNormParams& p, cudaStream_t st) {
-    const int chunks = p.D / EL;
-    const int sms = sm_count();
+int dispatch_add_norm(AddNormParams p, cudaStream_t st) {
+    const int chunks = p.D / EL, most = (chunks + 31) / 32, sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
-    // 64 elements per thread, as in the other row quantizers; with few rows as many threads per row as there are chunks.
-    int tpr = 32;
-    while (tpr < 256 && (tpr * 64 < p.D || (tpr < chunks && p.M * tpr < (int64_t)kThreads * sms))) tpr *= 2;
-    const int n = (chunks + tpr - 1) / tpr;
-    if (n <= 1) return launch_add_norm<EL, 1, kRowScale>(tpr, p, st);
-    if (n <= 2) return launch_add_norm<EL, 2, kRowScale>(tpr, p, st);
-    if (n <= 4) return launch_add_norm<EL, 4, kRowScale>(tpr, p, st);
-    if constexpr (EL == 8) {
-        if (n > 8) return launch_add_norm<EL, 16, kRowScale>(tpr, p, st);
+    int nw;
+    if (most == 1 || (most <= kMaxWarps && p.M * most <= 16 * (int64_t)sms)) nw = 1;
+    else if constexpr (EL == 16) nw = most <= 2 * kMaxWarps ? 2 : 4;
+    else nw = most <= 3 * 8 ? 3 : most <= 6 * 8 ? 6 : 8;
+    void (*kern)(AddNormParams) = add_rmsnorm_quant_kernel<EL, 1, kRowScale>;
+    if constexpr (EL == 16) {
+        if (nw == 2) kern = add_rmsnorm_quant_kernel<EL, 2, kRowScale>;
+        if (nw == 4) kern = add_rmsnorm_quant_kernel<EL, 4, kRowScale>;
+    } else {
+        if (nw == 3) kern = add_rmsnorm_quant_kernel<EL, 3, kRowScale>;
+        if (nw == 6) kern = add_rmsnorm_quant_kernel<EL, 6, kRowScale>;
+        if (nw == 8) kern = add_rmsnorm_quant_kernel<EL, 8, kRowScale>;
     }
-    return launch_add_norm<EL, 8, kRowScale>(tpr, p, st);        // D <= 32768: n <= 8 chunks of 16, n <= 16 of 8
+    p.warps = (most + nw - 1) / nw;                  // at most kMaxWarps: D <= 32768
+    const int teams = p.warps >= kThreads / 32 ? 1 : kThreads / 32 / p.warps;
+    HKB_CUDA(launch_dependent(true, kern, (unsigned)((p.M + teams - 1) / teams), 32 * p.warps * teams, 0, 0, st, p));
+    return check_launch("add_rmsnorm_quant_kernel");
 }
 
 // fp32 groups of 128 -> codes and scales: eight lanes per group, 16 elements each.
@@ -249,7 +246,7 @@ extern "C" int hkb_add_rmsnorm_quant_fp8(const void* x, const void* residual, co
                 HKB_ERR_BAD_ALIGN, "add_rmsnorm_quant_fp8: x, residual, w and residual_out must be 16-byte, q 8-byte, scales 4-byte aligned");
     if (M == 0) return HKB_OK;
     const AddNormParams p{(const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)w, (__nv_bfloat16*)residual_out,
-                          (uint8_t*)q, scales, M, (int)D, eps};
+                          (uint8_t*)q, scales, M, (int)D, eps, 0};
     // 32-byte chunks where every row of every tensor starts on one
     const bool wide = D % 16 == 0 && aligned32(x) && aligned32(residual) && aligned32(residual_out) && aligned16(q);
     cudaStream_t st = (cudaStream_t)stream;

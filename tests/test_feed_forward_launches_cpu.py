@@ -6,7 +6,7 @@ import shutil
 import subprocess
 import sys
 
-from test_launches_cpu import HKB_ERR_CUDA, ROOT, Runtime
+from test_launches_cpu import HKB_ERR_CUDA, LAUNCH, ROOT, Runtime
 
 i64, f32, i32 = ctypes.c_int64, ctypes.c_float, ctypes.c_int
 
@@ -28,15 +28,24 @@ def check_launches():
     def gated(M, F, K, fp8):
         return lambda: rt.lib.hkb_gemm_fp8_blockscale_gated(P[0], P[1], P[2], P[3] if fp8 else None, P[4], P[5], i32(4), P[6], i64(M), i64(F), i64(K), None)
 
-    # every row has its threads: grid * (256 / TPR) rows, TPR wide enough for D
+    # every row has its threads: a team of warps per row, `nw` chunks of `el` elements per thread, as many rows per CTA as teams
+    seen = []
+    with_block = LAUNCH(lambda name, grid, block, smem, cluster, early, args: seen.append((name.decode(), grid, block)) or 0)
+    rt.fake.fake_callbacks(with_block, *rt._keep[1:])
     for M in (1, 2, 3, 147, 148, 149, 1000, 16384, 2147483647):
-        for D in (8, 128, 136, 512, 1024, 2048, 4096, 4104, 8192, 16384, 16392, 32768):
+        for D in (8, 128, 136, 512, 1024, 1032, 2048, 4096, 4104, 5120, 8192, 16384, 16392, 32760, 32768):
             for group in {D, 128 if D % 128 == 0 else D}:
-                (name, grid, _), = launches(norm(M, D, group))
-                el, nw, tpr = (int(v) for v in name.split("add_rmsnorm_quant_kernelILi")[1].split("ELb")[0].split("ELi"))
-                assert el * nw * tpr >= D, (M, D, name)
-                assert grid * (256 // tpr) >= M and (grid - 1) * (256 // tpr) < M, (M, D, name, grid)
+                seen.clear()
+                assert norm(M, D, group)() == 0, rt.lib.hkb_last_error()
+                (name, grid, block), = seen
+                el, nw = (int(v) for v in name.split("add_rmsnorm_quant_kernelILi")[1].split("ELb")[0].split("ELi"))
                 assert el == (16 if D % 16 == 0 else 8)
+                chunks = D // el
+                warps = -(-(-(-chunks // 32)) // nw)
+                teams = max(1, 8 // warps)
+                assert warps <= 16 and block == 32 * warps * teams, (M, D, name, block)
+                assert grid == -(-M // teams), (M, D, name, grid)
+    rt.fake.fake_callbacks(*rt._keep)
     # gated: one launch, and a second one for a decode call's codes; shared memory within the limit
     for F, K in ((128, 128), (1152, 4224), (14336, 4096), (28672, 8192)):
         for M in (1, 16, 17, 32, 33, 128, 129, 4096):
