@@ -237,14 +237,14 @@ int launch_quant_f32_1x128(const float* y, void* q, float* scales, int64_t group
 extern "C" int hkb_add_rmsnorm_quant_fp8(const void* x, const void* residual, const void* w, void* q, float* scales, void* residual_out,
                                          int64_t M, int64_t D, int64_t group, float eps, void* stream) {
     using namespace hkb;
-    HKB_REQUIRE(x && residual && w && q && scales && residual_out, HKB_ERR_BAD_ARG, "add_rmsnorm_quant_fp8: null pointer");
     HKB_REQUIRE(M >= 0 && M <= 0x7FFFFFFFLL && D > 0 && D <= 32768 && D % 8 == 0, HKB_ERR_BAD_SHAPE,
                 "add_rmsnorm_quant_fp8: need D %% 8 == 0 and 0 < D <= 32768, got M=%lld D=%lld", (long long)M, (long long)D);
     HKB_REQUIRE(group == D || (group == 128 && D % 128 == 0), HKB_ERR_BAD_SHAPE,
                 "add_rmsnorm_quant_fp8: one scale per 128 columns (D %% 128 == 0) or per row, got group %lld of D=%lld", (long long)group, (long long)D);
+    if (M == 0) return HKB_OK;               // an empty tensor has no address
+    HKB_REQUIRE(x && residual && w && q && scales && residual_out, HKB_ERR_BAD_ARG, "add_rmsnorm_quant_fp8: null pointer");
     HKB_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(residual_out) && ((uintptr_t)q & 7) == 0 && ((uintptr_t)scales & 3) == 0,
                 HKB_ERR_BAD_ALIGN, "add_rmsnorm_quant_fp8: x, residual, w and residual_out must be 16-byte, q 8-byte, scales 4-byte aligned");
-    if (M == 0) return HKB_OK;
     const AddNormParams p{(const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)w, (__nv_bfloat16*)residual_out,
                           (uint8_t*)q, scales, M, (int)D, eps, 0};
     // 32-byte chunks where every row of every tensor starts on one

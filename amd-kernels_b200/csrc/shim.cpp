@@ -40,7 +40,7 @@ struct TView {
 // everything else -- subclasses, duck-typed objects -- keeps the general path.  Held for the life of the process, under the GIL.
 // A pass of quantizer + GEMM, general path / this: 128 x 1024 x 1024 29.7 / 13.6 us, row-major MXFP4 with multiply-add 35.7 / 28.7.
 struct Torch {
-    PyObject *data_ptr, *shape, *dtype, *is_contiguous, *is_cuda, *get_device;      // interned attribute names
+    PyObject *data_ptr, *shape, *dtype, *is_contiguous, *get_device;      // interned attribute names
     PyObject *tensor, *parameter;                                                   // types
     PyObject *current_raw_stream, *exchange_device, *maybe_exchange_device;         // torch._C functions, all three or none
     struct { PyObject* obj; std::string name; } dtypes[16];                         // torch.dtype objects are singletons
@@ -63,7 +63,6 @@ Torch* torch_cached() {
     n->shape = PyUnicode_InternFromString("shape");
     n->dtype = PyUnicode_InternFromString("dtype");
     n->is_contiguous = PyUnicode_InternFromString("is_contiguous");
-    n->is_cuda = PyUnicode_InternFromString("is_cuda");
     n->get_device = PyUnicode_InternFromString("get_device");
     n->tensor = py::object(mod.attr("Tensor")).release().ptr();
     n->parameter = py::object(mod.attr("nn").attr("Parameter")).release().ptr();
@@ -116,7 +115,7 @@ TView view_tensor(Torch& T, PyObject* t, const char* name, bool need_contiguous)
     if (need_contiguous && owned(PyObject_CallMethodNoArgs(t, T.is_contiguous)).ptr() != Py_True)
         fail(std::string(name) + ": tensor must be contiguous (row-major, inner stride 1)");
     v.name = name;
-    if (owned(PyObject_GetAttr(t, T.is_cuda)).ptr() == Py_True) v.device = owned(PyObject_CallMethodNoArgs(t, T.get_device)).cast<int>();
+    v.device = owned(PyObject_CallMethodNoArgs(t, T.get_device)).cast<int>();       // -1 for a CPU tensor
     return v;
 }
 

@@ -126,11 +126,11 @@ def fused_rmsnorm_fp8_quant_fwd(*args, **kwargs):
     return _call("fused_fp8_quant_tk", "fused_rmsnorm_fp8_quant_fwd", *args, **kwargs)
 
 
-def fused_add_rmsnorm_fp8_quant_fwd(*args, **kwargs):
+def fused_add_rmsnorm_fp8_quant_fwd(input, residual, weight, output, scales, residual_out, eps=1e-6):
     """(input, residual, weight, output [M,D], scales, residual_out, eps) -- not in the reference: adds
     ``input`` to the residual stream (``residual_out`` may be ``residual``), normalises the sum and
     quantizes it with one scale per 128 columns (``scales`` f32 [M,D/128]) or per row ([M,1])."""
-    return _call("fused_fp8_quant_tk", "fused_add_rmsnorm_fp8_quant_fwd", *args, **kwargs)
+    return _load("fused_fp8_quant_tk").fused_add_rmsnorm_fp8_quant_fwd(input, residual, weight, output, scales, residual_out, eps)
 
 
 def fused_rmsnorm_mxfp4_quant_fwd(*args, **kwargs):

@@ -122,6 +122,11 @@ def test_add_norm_row_scales(hk, M, D):
     check_norm(hk, *norm_case(M, D, M + D), D)
 
 
+def test_add_norm_of_no_rows(hk):
+    e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device=DEV)      # noqa: E731
+    hk.fused_add_rmsnorm_fp8_quant_fwd(e(0, 256), e(0, 256), torch.ones(256, device=DEV).bfloat16(), e(0, 256, dtype=E4M3), e(0, 2, dtype=torch.float32), e(0, 256), EPS)
+
+
 @pytest.mark.parametrize("group", [128, 1024])
 def test_add_norm_in_place_and_on_offset_views(hk, group):
     M, D = 19, 1024
