@@ -113,6 +113,8 @@ struct GemmParams {
     int skip_kblock;           // >= 0: the producer leaves this K block of its first tile unloaded (wait-limit probe only)
     const __nv_bfloat16* residual;   // kOut == 5: C = act(gemm + bias) + residual, [batch, M, N] or null
     int act;                   // kOut == 5, 6: HKB_ACT_*
+    int tile_first, tile_end;  // kOut 5, 6 of the block-scale kernels: the tiles of this launch
+    int more;                  //   and whether a launch with the remaining ones follows
     int split;                 // kSplitK: CTAs (a cluster of 2, 4 or 8) that share a tile, each with a part of K
     uint8_t* q_out;            // kOut == 6: codes [M, N/2] and scales [M, N/256] instead of C, or null
     float* q_scale;
@@ -371,10 +373,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     // is half (v - split_from) % 2 of tile split_from + (v - split_from) / 2.
     constexpr bool kSplit = kPair && !kBlockScale;
     const int all_tiles = tiles_per_batch * p.batch;
-    const int total_tiles = kSplit ? all_tiles + (all_tiles - p.split_from) : all_tiles;
+    constexpr bool kRange = kBlockScale && (kEpi || kGated);
+    const int total_tiles = kSplit ? all_tiles + (all_tiles - p.split_from) : kRange ? p.tile_end : all_tiles;
     auto tile_of = [&](int v) { return kSplit && v >= p.split_from ? p.split_from + (v - p.split_from) / 2 : v; };
     auto half_of = [&](int v) { return kSplit && v >= p.split_from ? (v - p.split_from) & 1 : -1; };      // -1: the whole tile
-    const int tile0 = kPair ? (int)(blockIdx.x >> 1) : kSplitK ? (int)blockIdx.x / split : (int)blockIdx.x;
+    const int tile0 = kPair ? (int)(blockIdx.x >> 1) : (kRange ? p.tile_first : 0) + (kSplitK ? (int)blockIdx.x / split : (int)blockIdx.x);
     const int tile_step = kPair ? (int)(gridDim.x >> 1) : kSplitK ? (int)gridDim.x / split : (int)gridDim.x;
     constexpr int TILE_M = kPair ? 2 * BM : BM;
 
@@ -398,6 +401,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         else tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
     }
     pdl_wait();      // nothing in global memory is touched before this
+    if (kRange && p.more) pdl_trigger();       // the launch behind this one sets up while this one computes
     tc_fence_before();
     __syncthreads();
     if constexpr (kPair) { __syncwarp(); cluster_sync_all(); }   // the partner's barriers and TMEM exist before anyone signals them
@@ -1219,7 +1223,7 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
     auto kern = gemm_fp8_kernel<BN, STAGES, kBlockScale, kGn128, false, AROWS, kOut, kSplitK>;
     // the attribute is per device; set it on every call (cheap) so multi-device processes work
     HKB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic));
-    const int tiles = p.m_blks * p.n_blks * p.batch;
+    const int tiles = kBlockScale && kOut >= 5 ? p.tile_end - p.tile_first : p.m_blks * p.n_blks * p.batch;
     const int sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
     const int grid = kSplitK ? tiles * p.split : tiles < sms ? tiles : sms;
@@ -1246,13 +1250,13 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
 // (per-token: it runs beside the next tile's main loop) or plus it (block scales: the accumulators are in its registers); what a wider
 // tile adds once, at the end; and for a split its barriers and exchange and a sixth on every K block.  The weights cannot come faster
 // than 5 TB/s.  The constants are fits of the figures at the two callers below.
-struct TilePlan { int bn, split; };
+struct TilePlan { int bn, split, tail; };          // tail: CTAs per tile of the last, partial wave (1: as the others)
 struct TileCost { int bn; double lone_us, full_us, least_us, wave_us, once_us, split_us; const void* split_kernel; int threads, smem; };
 template <int kN>
-TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K, int64_t batch, double* us_out = nullptr) {
+TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K, int64_t batch, bool tails, double* us_out = nullptr) {
     const int64_t sms = sm_count(), kblocks = K / BK;
     const double stream_us = (double)batch * N * K / 5e6;
-    TilePlan best{0, 1};
+    TilePlan best{0, 1, 1};
     double best_us = 1e30;
     for (const TileCost& c : costs) {
         if (c.bn == 0) continue;
@@ -1263,7 +1267,16 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
             const double loop = (kblocks + split - 1) / split * (c.lone_us + (c.full_us - c.lone_us) * busy) * (split > 1 ? 1.15 : 1.0);
             double us = waves * (loop > c.least_us ? loop : c.least_us);
             us = (us > stream_us ? us : stream_us) + waves * c.wave_us + c.once_us + (split > 1 ? c.split_us + 0.3 * split : 0);
-            if (us < best_us) { best_us = us; best = TilePlan{c.bn, split}; }
+            if (us < best_us) { best_us = us; best = TilePlan{c.bn, split, 1}; }
+        }
+        // Whole waves, then the tiles that are left in a launch of their own, split.  That launch costs about 10 us from the end of the one
+        // ahead of it to its own, so K has to be long: one launch / two, us, 4096 x 4096 x 14336 269 / 253, 2048 x 8192 x 8192 164 / 158, but
+        // 4096 x 14336 x 4096 291 / 297, 1024 x 14336 x 4096 82.8 / 84.6.
+        const int64_t left = tiles % sms;
+        for (int split = 2; tails && waves > 1 && left && split <= 8 && split <= kblocks && left * split <= sms; split *= 2) {
+            if (left > max_clusters(c.split_kernel, c.threads, c.smem, split)) break;
+            const double us = (waves - 1) * (kblocks * c.full_us + c.wave_us) + (kblocks + split - 1) / split * c.full_us * 1.15 + c.wave_us + c.split_us + 0.3 * split + 10;
+            if (us < best_us) { best_us = us; best = TilePlan{c.bn, 1, split}; }
         }
     }
     if (us_out) *us_out = best_us;
@@ -1280,7 +1293,27 @@ TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool narrow_ok, bool 
          SmemLayout<128, 5, false, BM, 128, 32, stage_out_bytes<128, kOut>()>::kDynamic},
         {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 2, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
          SmemLayout<256, 3, false, BM, 256, 32, stage_out_bytes<256, kOut>()>::kDynamic}};
-    return plan_tiles(costs, M, N, K, 1);
+    return plan_tiles(costs, M, N, K, 1, true);
+}
+
+// The launches of a plan: all tiles at once, whole or split, or the whole waves and behind them the rest, split.
+template <int BN, int STAGES, int kOut>
+int launch_block_scale(const CUtensorMap& tmA, const CUtensorMap& tmB, GemmParams p, const TilePlan& plan, cudaStream_t st) {
+    const int tiles = p.m_blks * p.n_blks;
+    p.tile_first = 0;
+    p.tile_end = tiles;
+    p.split = plan.split;
+    if (plan.split > 1) return launch_gemm<BN, STAGES, true, true, BM, kOut, true>(tmA, tmB, p, st);
+    if (plan.tail == 1) return launch_gemm<BN, STAGES, true, true, BM, kOut>(tmA, tmB, p, st);
+    p.tile_end = tiles - tiles % sm_count();
+    p.more = 1;
+    const int rc = launch_gemm<BN, STAGES, true, true, BM, kOut>(tmA, tmB, p, st);
+    if (rc != HKB_OK) return rc;
+    p.tile_first = p.tile_end;
+    p.tile_end = tiles;
+    p.more = 0;
+    p.split = plan.tail;
+    return launch_gemm<BN, STAGES, true, true, BM, kOut, true>(tmA, tmB, p, st);
 }
 
 int common_checks(const char* who, const void* A, const void* B, const void* C, int64_t batch, int64_t M, int64_t N, int64_t K) {
@@ -1378,7 +1411,7 @@ int launch_pts_epilogue(const void* A, const void* B, GemmParams p, cudaStream_t
                                {128, 0.22, 0.255, 3, 0, 1, 2.5, (const void*)gemm_fp8_kernel<128, 6, false, false, false, BM, 5, true>, gemm_threads<128, false>(), SmemLayout<128, 6>::kDynamic},
                                {256, 0.36, 0.413, 4.5, 0, 2.8, 0, nullptr, 0, 0}};      // not split: behind a narrower tile at every size tried
     double us = 0;
-    const TilePlan plan = plan_tiles(costs, M, N, K, batch, &us);
+    const TilePlan plan = plan_tiles(costs, M, N, K, batch, false, &us);
     // CTA pairs take 256 x 256 tiles, the last wave in halves where that is enough (launch_gemm_pair).  64 / 128 / 256-wide tiles / pairs,
     // us: 512 x 2048 x 1024 5.9 / 7.4 / 10.5 / 11.5, 512 x 4096 x 4096 16.1 / 12.6 / 19.4 / 19.1, 300 x 4096 x 14336 43.5 / 30.3 / 48.7 / 41.4,
     // 1024 x 14336 x 4096 84.7 / 65.0 / 62.2 / 55.5, 4096 x 4096 x 1024 29.9 / 24.8 / 24.5 / 21.8.  Split, whole / 2 / 4: 128 x 4096 x 14336
@@ -1607,10 +1640,10 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     const int sms = sm_count();
     int bn = 256;
     if (gn != 128 || sc || N % 256 != 0 || (int64_t)p.m_blks * (N / 256) < 2LL * sms) bn = 128;
+    TilePlan plan{};
     if (ep && gn == 128) {
-        const TilePlan plan = plan_block_scale<5>(M, N, K, true, N % 256 == 0);
+        plan = plan_block_scale<5>(M, N, K, true, N % 256 == 0);
         bn = plan.bn;
-        p.split = plan.split;
     }
     p.n_blks = (int)(N / bn);
     cudaStream_t st = (cudaStream_t)stream;
@@ -1647,10 +1680,9 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
         return launch_gemm<128, 5, true, true, BM, 1>(tmA, tmB, p, st);
     }
     if (ep) {
-        if (gn != 128) return launch_gemm<128, 6, true, false, BM, 5>(tmA, tmB, p, st);
-        if (p.split > 1) return bn == 256 ? launch_gemm<256, 3, true, true, BM, 5, true>(tmA, tmB, p, st) : launch_gemm<128, 5, true, true, BM, 5, true>(tmA, tmB, p, st);
-        if (bn == 256) return launch_gemm<256, 3, true, true, BM, 5>(tmA, tmB, p, st);
-        return launch_gemm<128, 5, true, true, BM, 5>(tmA, tmB, p, st);
+        if (gn == 128) return bn == 256 ? launch_block_scale<256, 3, 5>(tmA, tmB, p, plan, st) : launch_block_scale<128, 5, 5>(tmA, tmB, p, plan, st);
+        p.tile_end = p.m_blks * p.n_blks;
+        return launch_gemm<128, 6, true, false, BM, 5>(tmA, tmB, p, st);
     }
     if (gn == 128) {
         if (bn == 256) return launch_gemm<256, 3, true, true>(tmA, tmB, p, st);
@@ -1715,16 +1747,13 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     p.a_box_rows = BM;
     const TilePlan plan = plan_block_scale<6>(M, 2 * F, K, c_scale == nullptr, true);        // FP8: a tile has to hold whole scale groups
     const int bn = plan.bn;
-    p.split = plan.split;
     p.n_blks = (int)(F / (bn / 2));
     CUtensorMap tmA, tmB;
     rc = make_tmap_bytes(&tmA, A, (uint64_t)K, (uint64_t)M, 1, BM);
     if (rc != HKB_OK) return rc;
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)(2 * F), 1, (uint32_t)bn / 2);
     if (rc != HKB_OK) return rc;
-    if (p.split > 1) return bn == 256 ? launch_gemm<256, 3, true, true, BM, 6, true>(tmA, tmB, p, st) : launch_gemm<128, 5, true, true, BM, 6, true>(tmA, tmB, p, st);
-    if (bn == 256) return launch_gemm<256, 3, true, true, BM, 6>(tmA, tmB, p, st);
-    return launch_gemm<128, 5, true, true, BM, 6>(tmA, tmB, p, st);
+    return bn == 256 ? launch_block_scale<256, 3, 6>(tmA, tmB, p, plan, st) : launch_block_scale<128, 5, 6>(tmA, tmB, p, plan, st);
 }
 
 }  // extern "C"

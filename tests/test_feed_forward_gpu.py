@@ -252,6 +252,7 @@ def test_linear_per_token_kernels(hk, batch, M, N, K, kernel):
     (33, 1152, 384, 128, BLOCK(128, "")), (1025, 9728, 256, 128, BLOCK(128, "")),
     (300, 128, 5248, 128, BLOCK(128, ",split")), (40, 128, 8320, 128, BLOCK(128, ",split")),
     (1025, 9728, 1024, 128, BLOCK(256, "")), (300, 4096, 14336, 128, BLOCK(256, ",split")), (600, 1024, 8320, 128, BLOCK(256, ",split")),
+    (300, 14336, 4096, 128, BLOCK(256, ",split")), (2047, 8192, 8320, 128, BLOCK(256, ",split")),            # whole waves and a split rest
     (200, 256, 384, 1, BLOCK(128, "").replace("scale", "scale,gn1")), (3, 128, 128, 1, BLOCK(128, "").replace("scale", "scale,gn1"))])
 def test_linear_block_scale_kernels(hk, M, N, K, gn, kernel):
     check_linear(hk, "block", 1, M, N, K, act="gelu", gn=gn, kernel=kernel)
@@ -370,6 +371,7 @@ GATED = "gemm_fp8_kernel<{},blockscale,gated{}>".format
     (33, 128, 128, True, GATED(256, "")), (33, 128, 128, False, GATED(128, "")), (257, 640, 384, False, GATED(128, "")),
     (200, 640, 4224, False, GATED(128, ",split")), (130, 1024, 8192, False, GATED(128, ",split")), (40, 128, 8320, False, GATED(128, ",split")),
     (300, 1152, 4224, True, GATED(256, ",split")), (70, 256, 2048, True, GATED(256, ",split")), (40, 128, 8320, True, GATED(256, ",split")),
+    (512, 14336, 4096, True, GATED(256, ",split")), (500, 14336, 4224, False, GATED(256, ",split")),            # whole waves and a split rest
     (1025, 9600, 256, False, GATED(256, "")), (1300, 4096, 128, True, GATED(256, ""))])
 def test_gated_kernels(hk, M, F, K, fp8, kernel):
     check_gated(hk, M, F, K, "silu", fp8, kernel)
