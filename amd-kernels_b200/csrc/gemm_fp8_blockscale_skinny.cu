@@ -143,6 +143,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
     }
     if (warp == 1) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
     pdl_wait();      // nothing in global memory is touched before this
+    if constexpr (kOut != 0) pdl_trigger();  // the launch behind this one sets up while this one computes: 1 x 1024 x 1024 4.5 -> 3.9 us
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
