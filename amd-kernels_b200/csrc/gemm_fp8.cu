@@ -1262,21 +1262,26 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
         if (c.bn == 0) continue;
         const int64_t tiles = (M + BM - 1) / BM * ((N + c.bn - 1) / c.bn) * batch, waves = (tiles + sms - 1) / sms;
         for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
-            if (split > 1 && (!c.split_kernel || tiles * split > sms || tiles > max_clusters(c.split_kernel, c.threads, c.smem, split))) break;
+            if (split > 1 && (!c.split_kernel || tiles * split > sms)) break;
             const double busy = tiles * split < sms ? (double)(tiles * split) / sms : 1.0;
             const double loop = (kblocks + split - 1) / split * (c.lone_us + (c.full_us - c.lone_us) * busy) * (split > 1 ? 1.15 : 1.0);
             double us = waves * (loop > c.least_us ? loop : c.least_us);
             us = (us > stream_us ? us : stream_us) + waves * c.wave_us + c.once_us + (split > 1 ? c.split_us + 0.3 * split : 0);
-            if (us < best_us) { best_us = us; best = TilePlan{c.bn, split, 1}; }
+            if (us < best_us && (split == 1 || tiles <= max_clusters(c.split_kernel, c.threads, c.smem, split))) {
+                best_us = us;
+                best = TilePlan{c.bn, split, 1};
+            }
         }
         // Whole waves, then the tiles that are left in a launch of their own, split.  That launch costs about 10 us from the end of the one
         // ahead of it to its own, so K has to be long: one launch / two, us, 4096 x 4096 x 14336 269 / 253, 2048 x 8192 x 8192 164 / 158, but
         // 4096 x 14336 x 4096 291 / 297, 1024 x 14336 x 4096 82.8 / 84.6.
         const int64_t left = tiles % sms;
         for (int split = 2; tails && waves > 1 && left && split <= 8 && split <= kblocks && left * split <= sms; split *= 2) {
-            if (left > max_clusters(c.split_kernel, c.threads, c.smem, split)) break;
             const double us = (waves - 1) * (kblocks * c.full_us + c.wave_us) + (kblocks + split - 1) / split * c.full_us * 1.15 + c.wave_us + c.split_us + 0.3 * split + 10;
-            if (us < best_us) { best_us = us; best = TilePlan{c.bn, 1, split}; }
+            if (us < best_us && left <= max_clusters(c.split_kernel, c.threads, c.smem, split)) {
+                best_us = us;
+                best = TilePlan{c.bn, 1, split};
+            }
         }
     }
     if (us_out) *us_out = best_us;

@@ -484,7 +484,7 @@ void plan_split(bool nt16, const BsSkinnyOut& out, int64_t units, int parts, int
         return pull > hand_off ? pull : hand_off;
     };
     double best = rounds * ksteps * step_us((units + p.tiles - 1) / p.tiles);
-    for (int split = 2; split <= 8 && split <= ksteps; split *= 2) {
+    for (int split = 2; split <= 8 && split <= ksteps && best > 2; split *= 2) {
         const int64_t clusters = max_clusters(kern, kThreads, kSmemLimit, split);
         if (clusters == 0) break;
         const int64_t tiles = units < clusters ? units : clusters, height = (units + tiles - 1) / tiles;

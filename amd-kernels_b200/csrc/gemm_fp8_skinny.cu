@@ -369,7 +369,7 @@ gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 void plan_split(int units, int kblocks, int rounds, SkinnyParams& p) {
     auto block_us = [&](int width) { const double t = 0.12 + 0.021e-3 * (width * 2048 + p.a_bytes); return t > 0.17 ? t : 0.17; };
     double best = (double)rounds * kblocks * block_us((units + p.tiles - 1) / p.tiles);
-    for (int split = 2; split <= 8 && split <= kblocks; split *= 2) {
+    for (int split = 2; split <= 8 && split <= kblocks && best > 2.4; split *= 2) {
         const int clusters = max_clusters((const void*)gemm_fp8_skinny_kernel<true, true>, 192, kSmemLimit, split);
         if (clusters == 0) break;
         const int tiles = units < clusters ? units : clusters, width = (units + tiles - 1) / tiles;

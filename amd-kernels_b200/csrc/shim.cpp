@@ -20,19 +20,35 @@ namespace py = pybind11;
 
 namespace {
 
+[[noreturn]] void fail(const std::string& m) { throw std::runtime_error(m); }
+
+// A tensor's extents, in place: a vector per argument is an allocation per argument.
+struct Shape {
+    int64_t d[8];
+    int n = 0;
+    void push_back(int64_t v) {
+        if (n == 8) fail("tensors of more than 8 dimensions are not accepted");
+        d[n++] = v;
+    }
+    int size() const { return n; }
+    int64_t back() const { return d[n - 1]; }
+    int64_t at(int i) const {
+        if (i < 0 || i >= n) fail("tensor has too few dimensions");
+        return d[i];
+    }
+};
+
 struct TView {
     void* ptr = nullptr;
-    std::vector<int64_t> shape;
+    Shape shape;
     std::string dtype;   // "bfloat16", "float8_e4m3fn", "uint8", "float32", ...
     int device = -1;     // CUDA ordinal, -1 = not a CUDA tensor
     int64_t numel = 1;
     bool none = true;
     const char* name = "";
     int64_t dim(int i) const { return shape.at(i < 0 ? shape.size() + i : i); }
-    int rank() const { return (int)shape.size(); }
+    int rank() const { return shape.size(); }
 };
-
-[[noreturn]] void fail(const std::string& m) { throw std::runtime_error(m); }
 
 // What a call needs from torch, looked up once: through the general path below a pass of two calls spends about 30 us on
 // the host, most of it in attribute names built as strings, dtype reprs, a Python context manager and a Stream object per call.
@@ -95,10 +111,11 @@ TView view_tensor(Torch& T, PyObject* t, const char* name, bool need_contiguous)
     py::object shape = owned(PyObject_GetAttr(t, T.shape));
     const Py_ssize_t rank = PyTuple_Size(shape.ptr());
     if (rank < 0) throw py::error_already_set();
-    v.shape.resize((size_t)rank);
     for (Py_ssize_t i = 0; i < rank; ++i) {
-        v.shape[i] = py::reinterpret_borrow<py::object>(PyTuple_GET_ITEM(shape.ptr(), i)).cast<int64_t>();
-        v.numel *= v.shape[i];
+        const int64_t e = PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), i));
+        if (e == -1 && PyErr_Occurred()) throw py::error_already_set();
+        v.shape.push_back(e);
+        v.numel *= e;
     }
     py::object dtype = owned(PyObject_GetAttr(t, T.dtype));
     int d = 0;
@@ -423,10 +440,10 @@ int activation(const py::object& act) {
     static const struct { const char* name; int id; } table[] = {{"none", HKB_ACT_NONE}, {"relu", HKB_ACT_RELU}, {"gelu", HKB_ACT_GELU},
                                                                  {"gelu_tanh", HKB_ACT_GELU_TANH}, {"silu", HKB_ACT_SILU}};
     if (act.is_none()) return HKB_ACT_NONE;
-    const std::string s = py::str(act).cast<std::string>();
-    for (const auto& e : table)
-        if (s == e.name) return e.id;
-    fail("unknown activation '" + s + "' (want 'none', 'relu', 'gelu', 'gelu_tanh' or 'silu')");
+    if (PyUnicode_Check(act.ptr()))
+        for (const auto& e : table)
+            if (PyUnicode_CompareWithASCIIString(act.ptr(), e.name) == 0) return e.id;
+    fail("unknown activation '" + py::str(act).cast<std::string>() + "' (want 'none', 'relu', 'gelu', 'gelu_tanh' or 'silu')");
 }
 
 // Not in the reference: C = act(gemm + bias) + residual, per-token scales.  C may be residual itself.
