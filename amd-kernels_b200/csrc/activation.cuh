@@ -22,7 +22,7 @@ __device__ __forceinline__ float act_relu(float v) { return v < 0.0f ? 0.0f : v;
 // v * Phi(v), two values at a time on the packed fp32 pipe.  For a = |v|, Phi(-a) = erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) t P(t) with
 // t = 1 / (1 + 0.36 a): the scaled function is smooth in t on (0, 1], and P, of degree 6, is a minimax fit of its relative error over
 // 0 <= a <= 14 (8.7e-7; with the roundings 2^-19.5 for a <= 3, 2^-18.7 for a <= 6, 2^-17 at 13, where the exponent's argument rounds).
-// 2000 x 14336 x 4096 with bias, us: this 93, erfcf() 123 (its 50 instructions per value outlast the main loop), no activation 92.
+// 2000 x 14336 x 4096 with bias, us: this 98, erfcf() 118 (its 50 instructions per value outlast the main loop), no activation 95.
 __device__ __forceinline__ float2 act_gelu2(float2 v) {
     const float2 a = make_float2(fabsf(v.x), fabsf(v.y));
     const float2 d = __ffma2_rn(a, make_float2(0.36f, 0.36f), make_float2(1.0f, 1.0f));

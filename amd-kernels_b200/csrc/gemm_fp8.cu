@@ -647,6 +647,48 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     for (int c = 0; c < cols && col_base + c < p.N; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(rrow + col_base + c));
             };
             if constexpr (kEpi && !kBlockScale) prefetch_residual();
+            // kEpi: `n` columns from TMEM: scales (per-token), bias, activation, residual, store.  What it needs is there when it starts or
+            // comes a step ahead: weight scales and bias, four columns per lane, were fetched while the tile was computed and go round
+            // by shuffles, the residuals of the first step are in res_next.  With these loads inside the steps, each behind its own
+            // test, a step waited for memory four times over.
+            float4 sb_own = make_float4(0, 0, 0, 0);
+            uint2 bias_own = make_uint2(0, 0);
+            auto finish_columns = [&](uint32_t taddr, int n, float sa, uint4 (&res_next)[4]) {
+#pragma unroll 1
+                for (int c = 0; c < n; c += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(taddr + c, r);
+                    const int col0 = col_base + c;
+                    uint4 res[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) res[j] = res_next[j];
+                    if (c + 32 < n) load_residual<32, !kBlockScale>(rrow, col0 + 32, p.N, res_wide, res_next);
+                    tmem_ld_wait();
+                    float w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const int from = (c + j) >> 2;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[j + i] = __uint_as_float(r[j + i]);
+                        if constexpr (!kBlockScale) {
+                            w[j] = w[j] * sa * __shfl_sync(0xFFFFFFFFu, sb_own.x, from);
+                            w[j + 1] = w[j + 1] * sa * __shfl_sync(0xFFFFFFFFu, sb_own.y, from);
+                            w[j + 2] = w[j + 2] * sa * __shfl_sync(0xFFFFFFFFu, sb_own.z, from);
+                            w[j + 3] = w[j + 3] * sa * __shfl_sync(0xFFFFFFFFu, sb_own.w, from);
+                        }
+                    }
+                    if (p.bias) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, bias_own.x, (c + j) >> 2), b1 = __shfl_sync(0xFFFFFFFFu, bias_own.y, (c + j) >> 2);
+                            w[j] += bf16_lo(b0); w[j + 1] += bf16_hi(b0); w[j + 2] += bf16_lo(b1); w[j + 3] += bf16_hi(b1);
+                        }
+                    }
+                    apply_act<32>(w, p.act);
+                    if (p.residual) add_residual<32>(res, w);
+                    if (row_ok) store_row32(crow, col0, p.N, w, wide);
+                }
+            };
             // ---- split K ----
             // Slots in the operand rings: [rank of the sender][epilogue warp][16-byte chunk of the slice][lane].  A slice is COLS_PER_GROUP /
             // split columns of the warp (gated: half as many gate columns, then the up columns that go with them).
@@ -713,12 +755,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 const float sa = row_ok ? __ldg(p.sa + (int64_t)b * p.M + row) : 0.0f;
                 const float* sbp = p.sb + (int64_t)b * p.N;
                 const __nv_bfloat16* biasp = p.bias ? p.bias + (int64_t)b * p.N : nullptr;
-                // kEpi: scales and bias of the warp's columns, four per lane, are fetched while the tile is computed and go round by
-                // shuffles; the residuals are a 32-column step ahead.  With these loads inside the steps, each behind its own test, a
-                // step waited for memory four times over: 4096 x 4096 x 1024, us, plain epilogue 24.3 / 22.0, bias 25.5 / 23.8.  (Output turned
-                // through shared memory so that eight lanes store one row's 128 bytes: 24.1, 25.6, and gelu 42.8 instead of 32.)
-                float4 sb_own = make_float4(0, 0, 0, 0);
-                uint2 bias_own = make_uint2(0, 0);
                 uint4 res_next[4];
                 if constexpr (kEpi && !kSplitK) {
                     const int own = col_base + 4 * lane;
@@ -750,38 +786,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar(acc), acc_ph, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t t_addr = tmem_base + lane_addr + acc * BN + grp * cols;
+                if constexpr (kEpi) finish_columns(t_addr, cols, sa, res_next);
+                else
 #pragma unroll 1
                 for (int c = 0; c < cols; c += 32) {
                     uint32_t r[32];
                     tmem_ld32(t_addr + c, r);
                     const int col0 = col_base + c;
-                    if constexpr (kEpi) {
-                        uint4 res[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) res[j] = res_next[j];
-                        if (c + 32 < cols) load_residual<32, true>(rrow, col0 + 32, p.N, res_wide, res_next);
-                        tmem_ld_wait();
-                        float w[32];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const int from = (c + j) >> 2;
-                            w[j] = __uint_as_float(r[j]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.x, from);
-                            w[j + 1] = __uint_as_float(r[j + 1]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.y, from);
-                            w[j + 2] = __uint_as_float(r[j + 2]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.z, from);
-                            w[j + 3] = __uint_as_float(r[j + 3]) * sa * __shfl_sync(0xFFFFFFFFu, sb_own.w, from);
-                        }
-                        if (biasp) {
-#pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                const uint32_t b0 = __shfl_sync(0xFFFFFFFFu, bias_own.x, (c + j) >> 2), b1 = __shfl_sync(0xFFFFFFFFu, bias_own.y, (c + j) >> 2);
-                                w[j] += bf16_lo(b0); w[j + 1] += bf16_hi(b0); w[j + 2] += bf16_lo(b1); w[j + 3] += bf16_hi(b1);
-                            }
-                        }
-                        apply_act<32>(w, p.act);
-                        add_residual<32>(res, w);
-                        if (row_ok) store_row32(crow, col0, p.N, w, wide);
-                        continue;
-                    }
                     tmem_ld_wait();
                     float v[32];
 #pragma unroll
@@ -808,6 +819,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 // one scale per (row, K block) and per (K block, 128 columns): a single fp32 factor
                 // per thread and K block.  128 accumulators per thread as 64 float2 (packed FMA).
                 static_assert(COLS_PER_GROUP == 128, "block-scale epilogue groups own 128 columns");
+                if constexpr (kEpi && !kSplitK) {
+                    if (p.bias) bias_own = __ldg(reinterpret_cast<const uint2*>(p.bias + col_base + 4 * lane));
+                }
                 float2 acc2[64];
 #pragma unroll
                 for (int j = 0; j < 64; ++j) acc2[j] = make_float2(0.0f, 0.0f);
@@ -818,6 +832,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 // scales of the next chunk (32 K blocks; the next tile's first chunk at a tile's end)
                 // while this one is processed.
                 const int nchunks = (kbs + kScaleChunk - 1) / kScaleChunk;
+                constexpr bool kKeepLast = kEpi && !kSplitK;         // the epilogue uses the last K block's buffer
                 for (int ch = 0; ch < nchunks && ok; ++ch) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     __syncwarp();
@@ -875,7 +890,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc2[32 + j] = ffma2(ra[2 * j], ra[2 * j + 1], s2u, acc2[32 + j]);
                     tmem_ld_wait32(rb);
-                    release();
+                    if (!kKeepLast || ch < nchunks - 1 || kk < kb_end - 1) release();
                     if constexpr (kTrace) trace_at(4 + ew, ch * kScaleChunk + kk, lane == 0 && t == tile0 + 2 * tile_step, clock64());
 #pragma unroll
                     for (int j = 0; j < 16; ++j) acc2[48 + j] = ffma2(rb[2 * j], rb[2 * j + 1], s2u, acc2[48 + j]);
@@ -1010,23 +1025,23 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         }
                     }
                 } else if constexpr (kEpi) {
-                    if (ok && row_ok) {
+                    // The sums go back into the TMEM buffer of the last K block, which was not handed back, and come out again 32 columns at a
+                    // time in a short loop.  From the registers, which take no index, the epilogue is 128 columns of straight code, fetched
+                    // anew for every tile, with no register left for loads ahead.  4096 x 4096 x 1024, us, from TMEM and from registers: no
+                    // extras 33.3 and 35.3, bias 36.9 and 43.1, silu 40.0 and 45.3, bias + gelu + residual 53.1 and 60.5; 70 x 1024 x 128
+                    // with the three 7.3 and 9.4.
+                    if (!ok) break;
+                    const int buf = acc ^ 1;
+                    const uint32_t t_buf = tmem_base + lane_addr + buf * BN + grp * COLS_PER_GROUP;
 #pragma unroll
-                        for (int h = 0; h < 128; h += 64) {      // all residuals of 64 columns are in flight at once; 128 do not fit the registers
-                            uint4 res[8];
-                            load_residual<64, false>(rrow, col_base + h, p.N, res_wide, res);
-#pragma unroll
-                            for (int c = 0; c < 64; c += 16) {
-                                float v[16];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) { v[2 * i] = acc2[(h + c) / 2 + i].x; v[2 * i + 1] = acc2[(h + c) / 2 + i].y; }
-                                if (p.bias) add_bias<16>(p.bias, col_base + h + c, v);
-                                apply_act<16>(v, p.act);
-                                add_residual<16>(res + c / 8, v);
-                                store_bf16x16(crow + col_base + h + c, v);
-                            }
-                        }
-                    }
+                    for (int c = 0; c < 128; c += 32) tmem_st32(t_buf + c, reinterpret_cast<const float*>(acc2) + c);
+                    uint4 res_next[4];
+                    load_residual<32, false>(rrow, col_base, p.N, res_wide, res_next);
+                    tmem_st_wait();
+                    finish_columns(t_buf, 128, 1.0f, res_next);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar(buf));
                 } else if (ok && row_ok) {
                     // N % 128 == 0 in block-scale mode: rows are 32-byte aligned, whole groups are in range
 #pragma unroll
