@@ -112,11 +112,11 @@ struct GemmParams {
     uint64_t wait_ns;          // limit of every mbarrier wait (kWaitLimitNs in production)
     int skip_kblock;           // >= 0: the producer leaves this K block of its first tile unloaded (wait-limit probe only)
     const __nv_bfloat16* residual;   // kOut == 5: C = act(gemm + bias) + residual, [batch, M, N] or null
-    int act;                   // kOut == 5, 6: HKB_ACT_*
-    int tile_first, tile_end;  // kOut 5, 6 of the block-scale kernels: the tiles of this launch
+    int act;                   // kOut == 5, 6, 7: HKB_ACT_*
+    int tile_first, tile_end;  // kOut 5, 6, 7 of the block-scale kernels: the tiles of this launch
     int more;                  //   and whether a launch with the remaining ones follows
     int split;                 // kSplitK: CTAs (a cluster of 2, 4 or 8) that share a tile, each with a part of K
-    uint8_t* q_out;            // kOut == 6: codes [M, N/2] and scales [M, N/256] instead of C, or null
+    uint8_t* q_out;            // kOut == 7: codes [M, N/2] and scales [M, N/256] instead of C
     float* q_scale;
     unsigned long long* trace; // timeline build (kOut == 4) only: [grid][kTraceEvents][kTraceKb] SM clock readings
 };
@@ -290,11 +290,11 @@ __device__ __forceinline__ float2 ffma2(uint32_t a0, uint32_t a1, float2 s, floa
     return __ffma2_rn(make_float2(__uint_as_float(a0), __uint_as_float(a1)), s, c);
 }
 
-// Shared memory behind the scales.  kOut == 1: 32 rows x 128 bytes per epilogue warp.  kOut == 6: the up projection's weight scales
-// (as many as the gate's), row maxima of the eight epilogue warps for two tiles, four barriers for each of the two.
+// Shared memory behind the scales.  kOut == 1: 32 rows x 128 bytes per epilogue warp.  kOut 6 and 7: the up projection's weight scales
+// (as many as the gate's); kOut == 7: row maxima of the eight epilogue warps for two tiles, four barriers for each of the two.
 constexpr int kGatedSbBytes = 2 * 8 * 32 * 4, kGatedMaxBytes = 2 * 8 * 32 * 4;
 template <int BN, int kOut>
-constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 : kOut == 6 ? kGatedSbBytes + kGatedMaxBytes + 8 * 8 : 0; }
+constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 : kOut == 7 ? kGatedSbBytes + kGatedMaxBytes + 8 * 8 : kOut == 6 ? kGatedSbBytes : 0; }
 
 // kOut (block-scale): 0 = plain [M, N] result; 1 = the result also goes to p.n_peer further destinations
 // (the other GPUs' copies of the assembled output; 128-column weight-scale groups only); 2 = split-cat;
@@ -304,9 +304,9 @@ constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 
 // kOut (both scale schemes): 5 = bias, activation and residual: C = act(gemm + bias) + residual.
 // kOut (block-scale, 128-column weight-scale groups): 6 = gated: the BN rows of a B tile are BN/2 gate rows and the BN/2 up rows of
 // the same output columns (two boxes, no re-ordering of the weights), and the tile gives BN/2 columns act(gate) * up.  A thread
-// promotes 64 gate and the 64 matching up columns, so the product needs nobody else; with FP8 output the two warps of a row
-// exchange one maximum through shared memory (BN = 256: a tile is exactly one 128-column scale group of the result).
-// kSplitK (kOut 5 and 6): a cluster of p.split CTAs has exactly one tile, each CTA a part of K.  At the end every epilogue warp writes
+// promotes 64 gate and the 64 matching up columns, so the product needs nobody else; 7 = gated with FP8 output: the two warps of a
+// row exchange one maximum through shared memory (BN = 256: a tile is exactly one 128-column scale group of the result).
+// kSplitK (kOut 5, 6 and 7): a cluster of p.split CTAs has exactly one tile, each CTA a part of K.  At the end every epilogue warp writes
 // its sums, a slice of its columns to each CTA of the cluster, into the operand rings (idle by then) through distributed shared
 // memory, and finishes its own slice: the parts added in the order of their ranks, so the result is the same every time, and every
 // warp of every CTA has a share of the epilogue.  The cluster barriers around that are reached by every thread on every path, an
@@ -321,9 +321,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     using L = SmemLayout<BN, STAGES, kPair, AROWS, (kBlockScale && kGn128) ? 128 * EPI_GROUPS : 0, kScaleChunk, kStageOut>;
     constexpr bool kGrouped = kOut == 3;
     constexpr bool kTrace = kOut == 4;
-    static_assert(!kSplitK || EPI_GROUPS * 4 * (BN / EPI_GROUPS) * 128 + (kOut == 6 ? 8 * 8 * 32 * 4 : 0) <= STAGES * L::kStageBytes, "split K: slots in the operand ring");
+    static_assert(!kSplitK || EPI_GROUPS * 4 * (BN / EPI_GROUPS) * 128 + (kOut == 7 ? 8 * 8 * 32 * 4 : 0) <= STAGES * L::kStageBytes, "split K: slots in the operand ring");
     constexpr bool kEpi = kOut == 5;
-    constexpr bool kGated = kOut == 6;
+    constexpr bool kGated = kOut == 6 || kOut == 7, kCodes = kOut == 7;
+    static_assert(!kCodes || BN == 256, "FP8 output: a tile is one scale group per row");
     static_assert(!kGated || (kBlockScale && kGn128 && !kPair), "gated mode: block scales, 128-column groups, one CTA");
     static_assert(!kGrouped || (kBlockScale && kGn128 && !kPair), "grouped mode: block scales, 128-column groups, one CTA");
     static_assert(!kPair || BN == 256, "CTA pairs work on 256 x 256 tiles");
@@ -391,7 +392,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             mbar_init(tempty_bar(a), kRelay ? 2 : kPair ? 2 * EPI_WARPS : EPI_WARPS);   // the leader hears both CTAs' epilogues
             mbar_init(relay_bar(a), EPI_WARPS);
         }
-        if constexpr (kGated)
+        if constexpr (kCodes)
             for (int i = 0; i < 8; ++i) mbar_init(max_bar(i), 2);
         *abort_flag = 0;
         fence_barrier_init();
@@ -832,7 +833,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 // scales of the next chunk (32 K blocks; the next tile's first chunk at a tile's end)
                 // while this one is processed.
                 const int nchunks = (kbs + kScaleChunk - 1) / kScaleChunk;
-                constexpr bool kKeepLast = kEpi && !kSplitK;         // the epilogue uses the last K block's buffer
+                constexpr int kHalf2 = kGated ? BN / 2 : 64;         // where the second 64 columns of a thread start
+                constexpr bool kKeepLast = (kEpi || kGated) && !kSplitK;         // the epilogue uses the last K block's buffer
                 for (int ch = 0; ch < nchunks && ok; ++ch) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     __syncwarp();
@@ -863,7 +865,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tc_fence_after();
                     if constexpr (kTrace) trace_at(12 + ew, ch * kScaleChunk + kk, lane == 0 && t == tile0 + 2 * tile_step, clock64());
                     const uint32_t t_addr = tmem_base + lane_addr + acc * BN + grp * (kGated ? 64 : COLS_PER_GROUP);
-                    constexpr int kHalf2 = kGated ? BN / 2 : 64;           // where the second 64 columns start
                     uint32_t ra[32], rb[32];
                     // the partial product lives in registers after the fourth load: the TMEM buffer goes back
                     // to the MMA thread before the last FMAs
@@ -918,7 +919,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             for (int k = 0; k < 8; ++k) y[k] *= up[k];
                         };
                         const bool mine = ok && any_rows;
-                        if (BN == 256 && p.q_out) {
+                        if constexpr (kCodes) {
                             // the row's maximum: every warp tells every CTA its own (behind the slots of the sums)
                             float* const maxima = reinterpret_cast<float*>(smem + EPI_WARPS * COLS_PER_GROUP * 128);      // [rank][warp][lane]
                             float am = 0.0f, y[8];
@@ -981,20 +982,47 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             __syncwarp();
                         }
                     }
-                } else if constexpr (kGated) {
-                    if (ok) {
-                        float* const y = reinterpret_cast<float*>(acc2);
+                } else if constexpr (kEpi || kGated) {
+                    // The sums go back into the TMEM buffer of the last K block, which was not handed back, and come out again 32 columns at a
+                    // time in a short loop.  From the registers, which take no index, the epilogue is 128 columns of straight code, fetched
+                    // anew for every tile, with no register left for loads ahead.  4096 x 4096 x 1024, us, from TMEM and from registers: no
+                    // extras 33.3 and 35.3, bias 36.9 and 43.1, silu 40.0 and 45.3, bias + gelu + residual 53.1 and 60.5; 70 x 1024 x 128
+                    // with the three 7.3 and 9.4; gated 2048 x 4096 x 1024 28.8 and 35.1, to codes 30.6 and 34.8.  Most of the gated gain is
+                    // the main loop's: with less live across it, it no longer spills.
+                    if (!ok) break;
+                    const int buf = acc ^ 1;
+                    const uint32_t t_buf = tmem_base + lane_addr + buf * BN + grp * (kGated ? 64 : COLS_PER_GROUP);
 #pragma unroll
-                        for (int j = 0; j < 64; j += 16) {
-                            apply_act<16>(y + j, p.act);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[j + i] *= y[64 + j + i];
-                        }
+                    for (int c = 0; c < 64; c += 32) {
+                        tmem_st32(t_buf + c, reinterpret_cast<const float*>(acc2) + c);
+                        tmem_st32(t_buf + kHalf2 + c, reinterpret_cast<const float*>(acc2) + 64 + c);
+                    }
+                    if constexpr (kGated) {
                         const int F = p.N / 2, out0 = nb * (BN / 2) + grp * 64;
-                        if (BN == 256 && p.q_out) {
-                            float am = 0.0f;
+                        float am = 0.0f;
+                        tmem_st_wait();
+#pragma unroll 1
+                        for (int c = 0; c < 64; c += 32) {
+                            uint32_t g[32], u[32];
+                            tmem_ld32(t_buf + c, g);
+                            tmem_ld32(t_buf + kHalf2 + c, u);
+                            tmem_ld_wait();
+                            float y[32];
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) am = max_nan(am, fabsf(y[j]));
+                            for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(g[i]);
+                            apply_act<32>(y, p.act);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] *= __uint_as_float(u[i]);
+                            if constexpr (kCodes) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) am = max_nan(am, fabsf(y[i]));
+                                tmem_st32(t_buf + c, y);
+                            } else if (row_ok) {
+                                store_bf16x16(p.C + (int64_t)row * F + out0 + c, y);
+                                store_bf16x16(p.C + (int64_t)row * F + out0 + c + 16, y + 16);
+                            }
+                        }
+                        if constexpr (kCodes) {
                             // the other half of the row is the other warp's; the two tiles' worth of slots alternate: a warp is back
                             // at a slot only after its partner has read it, since in between it waits for the partner's next maximum
                             float* const slots = reinterpret_cast<float*>(smem + L::kStageOutOffset + kGatedSbBytes) + (max_n & 1) * 256;
@@ -1002,43 +1030,33 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             slots[ew * 32 + lane] = am;
                             __syncwarp();
                             if (lane == 0) mbar_arrive(xb);
+                            tmem_st_wait();
                             if (!__all_sync(0xFFFFFFFFu, mbar_wait(xb, (max_n >> 1) & 1, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
                             am = max_nan(am, slots[(ew ^ 4) * 32 + lane]);
                             ++max_n;
                             const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f), rs = __frcp_rn(scale);
-                            if (row_ok) {
-                                uint32_t o[16];
+#pragma unroll 1
+                            for (int c = 0; c < 64; c += 32) {
+                                uint32_t y[32], o[8];
+                                tmem_ld32(t_buf + c, y);
+                                tmem_ld_wait();
 #pragma unroll
-                                for (int j = 0; j < 16; ++j)
-                                    o[j] = (uint32_t)cvt_e4m3x2(y[4 * j] * rs, y[4 * j + 1] * rs) | ((uint32_t)cvt_e4m3x2(y[4 * j + 2] * rs, y[4 * j + 3] * rs) << 16);
-                                uint8_t* const dst = p.q_out + (int64_t)row * F + out0;
-#pragma unroll
-                                for (int j = 0; j < 16; j += 8)
+                                for (int j = 0; j < 8; ++j)
+                                    o[j] = (uint32_t)cvt_e4m3x2(__uint_as_float(y[4 * j]) * rs, __uint_as_float(y[4 * j + 1]) * rs) |
+                                           ((uint32_t)cvt_e4m3x2(__uint_as_float(y[4 * j + 2]) * rs, __uint_as_float(y[4 * j + 3]) * rs) << 16);
+                                if (row_ok)
                                     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                                                 ::"l"(dst + 4 * j), "r"(o[j]), "r"(o[j + 1]), "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]), "r"(o[j + 5]),
-                                                   "r"(o[j + 6]), "r"(o[j + 7]) : "memory");
-                                if (grp == 0) p.q_scale[(int64_t)row * (F / 128) + nb] = scale;
+                                                 ::"l"(p.q_out + (int64_t)row * F + out0 + c), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]),
+                                                   "r"(o[6]), "r"(o[7]) : "memory");
                             }
-                        } else if (row_ok) {
-#pragma unroll
-                            for (int j = 0; j < 64; j += 16) store_bf16x16(p.C + (int64_t)row * F + out0 + j, y + j);
+                            if (row_ok && grp == 0) p.q_scale[(int64_t)row * (F / 128) + nb] = scale;
                         }
+                    } else {
+                        uint4 res_next[4];
+                        load_residual<32, false>(rrow, col_base, p.N, res_wide, res_next);
+                        tmem_st_wait();
+                        finish_columns(t_buf, 128, 1.0f, res_next);
                     }
-                } else if constexpr (kEpi) {
-                    // The sums go back into the TMEM buffer of the last K block, which was not handed back, and come out again 32 columns at a
-                    // time in a short loop.  From the registers, which take no index, the epilogue is 128 columns of straight code, fetched
-                    // anew for every tile, with no register left for loads ahead.  4096 x 4096 x 1024, us, from TMEM and from registers: no
-                    // extras 33.3 and 35.3, bias 36.9 and 43.1, silu 40.0 and 45.3, bias + gelu + residual 53.1 and 60.5; 70 x 1024 x 128
-                    // with the three 7.3 and 9.4.
-                    if (!ok) break;
-                    const int buf = acc ^ 1;
-                    const uint32_t t_buf = tmem_base + lane_addr + buf * BN + grp * COLS_PER_GROUP;
-#pragma unroll
-                    for (int c = 0; c < 128; c += 32) tmem_st32(t_buf + c, reinterpret_cast<const float*>(acc2) + c);
-                    uint4 res_next[4];
-                    load_residual<32, false>(rrow, col_base, p.N, res_wide, res_next);
-                    tmem_st_wait();
-                    finish_columns(t_buf, 128, 1.0f, res_next);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tempty_bar(buf));
@@ -1131,7 +1149,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             __syncwarp();
             cluster_sync_all();
             cluster_sync_all();
-            if (kGated && BN == 256 && p.q_out) cluster_sync_all();
+            if (kCodes) cluster_sync_all();
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");      // no staged-scale copy may outlive the CTA
@@ -1254,13 +1272,13 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
                 kOut == 4 ? "gemm_fp8_kernel<256,blockscale,timeline>" :
                 kOut == 5 ? (kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,epilogue>" : kGn128 ? "gemm_fp8_kernel<128,blockscale,epilogue>" : "gemm_fp8_kernel<128,blockscale,gn1,epilogue>")
                                          : (BN == 256 ? "gemm_fp8_kernel<256,pts,epilogue>" : BN == 128 ? "gemm_fp8_kernel<128,pts,epilogue>" : "gemm_fp8_kernel<64,pts,epilogue>")) :
-                kOut == 6 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,gated>" : "gemm_fp8_kernel<128,blockscale,gated>") :
+                kOut >= 6 ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,gated>" : "gemm_fp8_kernel<128,blockscale,gated>") :
                 kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale>" : kGn128 ? "gemm_fp8_kernel<128,blockscale>" : "gemm_fp8_kernel<128,blockscale,gn1>")
                             : (BN == 256 ? "gemm_fp8_kernel<256,pts>" : BN == 128 ? "gemm_fp8_kernel<128,pts>" : "gemm_fp8_kernel<64,pts>"));
     return check_launch("gemm_fp8_kernel");
 }
 
-// Tile width and CTAs per tile of the kernels with an epilogue of their own (kOut 5, 6).  All tiles take the same time, so what counts
+// Tile width and CTAs per tile of the kernels with an epilogue of their own (kOut 5, 6, 7).  All tiles take the same time, so what counts
 // is waves x (K blocks per CTA x the time of one, which grows with the share of the SMs at work), at least the time of the epilogue
 // (per-token: it runs beside the next tile's main loop) or plus it (block scales: the accumulators are in its registers); what a wider
 // tile adds once, at the end; and for a split its barriers and exchange and a sixth on every K block.  The weights cannot come faster
@@ -1307,9 +1325,11 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
 // 10.5 / 11.9 / 11.6; x 2048 12.8 / 11.8 / 10.2, 16.2 / 14.8 / 12.9; x 14336 49.0 / 32.4 / 21.9, 70.4 / 42.0 / 28.1; 128 x 1024 x 8192
 // 29.8 / 20.9 / 13.9 (11.0), 40.1 / 26.5 / 18.1 (15.7); 512 x 4096 x 4096 19.9, 25.6 / 21.0; 300 x 14336 x 4096 52.5, 50.1.
 template <int kOut>
-TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool narrow_ok, bool wide_ok) {
+TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool wide_ok) {
+    const void* narrow = nullptr;          // FP8 output: a tile has to hold whole scale groups
+    if constexpr (kOut != 7) narrow = (const void*)gemm_fp8_kernel<128, 5, true, true, false, BM, kOut, true>;
     const TileCost costs[2] = {
-        {narrow_ok ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, (const void*)gemm_fp8_kernel<128, 5, true, true, false, BM, kOut, true>, gemm_threads<128, true>(),
+        {narrow ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, narrow, gemm_threads<128, true>(),
          SmemLayout<128, 5, false, BM, 128, 32, stage_out_bytes<128, kOut>()>::kDynamic},
         {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 2, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
          SmemLayout<256, 3, false, BM, 256, 32, stage_out_bytes<256, kOut>()>::kDynamic}};
@@ -1662,7 +1682,7 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
     if (gn != 128 || sc || N % 256 != 0 || (int64_t)p.m_blks * (N / 256) < 2LL * sms) bn = 128;
     TilePlan plan{};
     if (ep && gn == 128) {
-        plan = plan_block_scale<5>(M, N, K, true, N % 256 == 0);
+        plan = plan_block_scale<5>(M, N, K, N % 256 == 0);
         bn = plan.bn;
     }
     p.n_blks = (int)(N / bn);
@@ -1765,7 +1785,7 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     p.wait_ns = kWaitLimitNs; p.skip_kblock = -1; p.status = status;
     p.m_blks = (int)((M + BM - 1) / BM);
     p.a_box_rows = BM;
-    const TilePlan plan = plan_block_scale<6>(M, 2 * F, K, c_scale == nullptr, true);        // FP8: a tile has to hold whole scale groups
+    const TilePlan plan = c_scale ? plan_block_scale<7>(M, 2 * F, K, true) : plan_block_scale<6>(M, 2 * F, K, true);
     const int bn = plan.bn;
     p.n_blks = (int)(F / (bn / 2));
     CUtensorMap tmA, tmB;
@@ -1773,6 +1793,7 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     if (rc != HKB_OK) return rc;
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)(2 * F), 1, (uint32_t)bn / 2);
     if (rc != HKB_OK) return rc;
+    if (c_scale) return launch_block_scale<256, 3, 7>(tmA, tmB, p, plan, st);
     return bn == 256 ? launch_block_scale<256, 3, 6>(tmA, tmB, p, plan, st) : launch_block_scale<128, 5, 6>(tmA, tmB, p, plan, st);
 }
 
