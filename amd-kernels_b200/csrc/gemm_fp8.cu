@@ -649,8 +649,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             };
             if constexpr (kEpi && !kBlockScale) prefetch_residual();
             // kEpi: `n` columns from TMEM: scales (per-token), bias, activation, residual, store.  What it needs is there when it starts or
-            // comes a step ahead: weight scales and bias, four columns per lane, were fetched while the tile was computed and go round
-            // by shuffles, the residuals of the first step are in res_next.  With these loads inside the steps, each behind its own
+            // comes a step ahead: weight scales and bias, four columns per lane, are fetched before (per-token while the tile is
+            // computed; block scales after it, or the main loop spills: 32.0 and 33.3 us at 4096 x 4096 x 1024) and go round by
+            // shuffles, the residuals of the first step are in res_next.  With these loads inside the steps, each behind its own
             // test, a step waited for memory four times over.
             float4 sb_own = make_float4(0, 0, 0, 0);
             uint2 bias_own = make_uint2(0, 0);
@@ -820,9 +821,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 // one scale per (row, K block) and per (K block, 128 columns): a single fp32 factor
                 // per thread and K block.  128 accumulators per thread as 64 float2 (packed FMA).
                 static_assert(COLS_PER_GROUP == 128, "block-scale epilogue groups own 128 columns");
-                if constexpr (kEpi && !kSplitK) {
-                    if (p.bias) bias_own = __ldg(reinterpret_cast<const uint2*>(p.bias + col_base + 4 * lane));
-                }
                 float2 acc2[64];
 #pragma unroll
                 for (int j = 0; j < 64; ++j) acc2[j] = make_float2(0.0f, 0.0f);
@@ -987,8 +985,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     // time in a short loop.  From the registers, which take no index, the epilogue is 128 columns of straight code, fetched
                     // anew for every tile, with no register left for loads ahead.  4096 x 4096 x 1024, us, from TMEM and from registers: no
                     // extras 33.3 and 35.3, bias 36.9 and 43.1, silu 40.0 and 45.3, bias + gelu + residual 53.1 and 60.5; 70 x 1024 x 128
-                    // with the three 7.3 and 9.4; gated 2048 x 4096 x 1024 28.8 and 35.1, to codes 30.6 and 34.8.  Most of the gated gain is
-                    // the main loop's: with less live across it, it no longer spills.
+                    // with the three 7.3 and 9.4; gated 2048 x 4096 x 1024 28.8 and 35.1, to codes 30.6 and 34.8 (with both outputs in one kernel, which
+                    // spills in its main loop, 32.8 and 34.7).
                     if (!ok) break;
                     const int buf = acc ^ 1;
                     const uint32_t t_buf = tmem_base + lane_addr + buf * BN + grp * (kGated ? 64 : COLS_PER_GROUP);
@@ -1054,6 +1052,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     } else {
                         uint4 res_next[4];
                         load_residual<32, false>(rrow, col_base, p.N, res_wide, res_next);
+                        if (p.bias) bias_own = __ldg(reinterpret_cast<const uint2*>(p.bias + col_base + 4 * lane));
                         tmem_st_wait();
                         finish_columns(t_buf, 128, 1.0f, res_next);
                     }
