@@ -323,6 +323,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     constexpr bool kTrace = kOut == 4;
     static_assert(!kSplitK || EPI_GROUPS * 4 * (BN / EPI_GROUPS) * 128 + (kOut == 7 ? 8 * 8 * 32 * 4 : 0) <= STAGES * L::kStageBytes, "split K: slots in the operand ring");
     constexpr bool kEpi = kOut == 5;
+    // With 128 sums and a partial product in its registers the main loop has none to spare, and spills, even outside its steps, cost a
+    // tile about 0.5 us.  So the rows' addresses and the bias are worked out and fetched behind it (kLate), and a narrow tile stages
+    // its scales in a rolled loop: 300 x 4096 x 1024 7.1 and 7.5 us, gated (F = 2048) 6.8 and 7.6, split 70 x 4096 x 2048 8.9 and 9.4.
+    constexpr bool kLate = kEpi && kBlockScale && kGn128;
     constexpr bool kGated = kOut == 6 || kOut == 7, kCodes = kOut == 7;
     static_assert(!kCodes || BN == 256, "FP8 output: a tile is one scale group per row");
     static_assert(!kGated || (kBlockScale && kGn128 && !kPair), "gated mode: block scales, 128-column groups, one CTA");
@@ -568,7 +572,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // float4 slots [kb/4][thread], and lane l of each warp the weight scale of K block l of the
         // warp's column group.  Completion is awaited by the same thread (sa) / warp (sb) only.
         auto stage_scales = [&](int buf, int tile, int chunk) {
-            const int tb = tile / tiles_per_batch;
+            const int tb = kLate ? 0 : tile / tiles_per_batch;
             int tmb, tnb;
             tile_coords(tile - tb * tiles_per_batch, p.m_blks, p.n_blks, kPair ? GROUP_M / 2 : GROUP_M, tmb, tnb);
             int r = tmb * TILE_M + (int)rank * BM + row_in_tile;
@@ -583,7 +587,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const float* src = p.sa + (int64_t)r * all_kblocks + k_begin + kb0;
             const uint32_t dst = smem_u32(sa_slots + (size_t)buf * (kScaleChunk / 4) * EPI_THREADS);
             const bool vec = (kblocks % 4) == 0 && (k_begin % 4) == 0 && (all_kblocks % 4) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
-#pragma unroll
+#pragma unroll (kOut >= 5 && BN == 128 ? 2 : 8)
             for (int j = 0; j < kScaleChunk / 4; ++j) {
                 const int kb = kb0 + 4 * j;
                 const uint32_t d = dst + (uint32_t)j * EPI_THREADS * 16;
@@ -624,7 +628,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
         for (int t = next_live_tile(tile0); t < total_tiles && ok; t = next_live_tile(t + tile_step)) {
             const int tt = tile_of(t), half = half_of(t);
-            const int b = tt / tiles_per_batch;
+            const int b = kLate ? 0 : tt / tiles_per_batch;
             int mb, nb;
             tile_coords(tt - b * tiles_per_batch, p.m_blks, p.n_blks, kPair ? GROUP_M / 2 : GROUP_M, mb, nb);
             int row = mb * TILE_M + (int)rank * BM + row_in_tile;
@@ -638,14 +642,20 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             }
             const int cols = half < 0 ? COLS_PER_GROUP : COLS_PER_GROUP / 2;
             const int col_base = nb * BN + (half < 0 ? grp * COLS_PER_GROUP : half * (BN / 2) + grp * (COLS_PER_GROUP / 2));
-            __nv_bfloat16* crow = p.C + ((int64_t)b * p.M + (row_ok ? row : 0)) * p.ldc;
-            const __nv_bfloat16* rrow = kEpi && p.residual && row_ok ? p.residual + ((int64_t)b * p.M + row) * p.N : nullptr;
+            __nv_bfloat16* crow;
+            const __nv_bfloat16* rrow;
+            auto set_rows = [&]() {
+                crow = p.C + ((int64_t)b * p.M + (row_ok ? row : 0)) * p.ldc;
+                rrow = kEpi && p.residual && row_ok ? p.residual + ((int64_t)b * p.M + row) * p.N : nullptr;
+            };
+            if constexpr (!kLate) set_rows();
             const bool res_wide = kEpi && (p.N % 16) == 0 && (reinterpret_cast<uintptr_t>(p.residual) & 31) == 0;
             // the row's residuals go towards L2 a few K blocks before they are needed (at the tile's start they would be gone again
             // from L2 by its end, behind the operands of a long K)
             auto prefetch_residual = [&]() {
-                if (rrow)
-                    for (int c = 0; c < cols && col_base + c < p.N; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(rrow + col_base + c));
+                if (p.residual && row_ok)
+                    for (int c = 0; c < cols && col_base + c < p.N; c += 64)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + ((int64_t)b * p.M + row) * p.N + col_base + c));
             };
             if constexpr (kEpi && !kBlockScale) prefetch_residual();
             // kEpi: `n` columns from TMEM: scales (per-token), bias, activation, residual, store.  What it needs is there when it starts or
@@ -717,13 +727,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             float4 sl_sb = make_float4(1, 1, 1, 1);
             uint2 sl_bias = make_uint2(0, 0);
             float sl_sa = 1.0f;
-            if constexpr (kSplitK && kEpi) {
+            auto fetch_slice = [&]() {
                 if (lane < nchunk && slice0 + 4 * lane < p.N) {
                     if constexpr (!kBlockScale) sl_sb = __ldg(reinterpret_cast<const float4*>(p.sb + (int64_t)b * p.N + slice0 + 4 * lane));
                     if (p.bias) sl_bias = __ldg(reinterpret_cast<const uint2*>(p.bias + (int64_t)b * p.N + slice0 + 4 * lane));
                 }
                 if (!kBlockScale && row_ok) sl_sa = __ldg(p.sa + (int64_t)b * p.M + row);
-            }
+            };
+            if constexpr (kSplitK && kEpi && !kLate) fetch_slice();
             auto finish_slice = [&]() {                                          // kEpi: bias, activation, residual, store
                 uint4 next[1];
                 load_residual<8, true>(rrow, slice0, p.N, false, next);
@@ -903,6 +914,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                         for (int j = 0; j < 32; ++j) send_part(j, acc2[2 * j].x, acc2[2 * j].y, acc2[2 * j + 1].x, acc2[2 * j + 1].y);
                     }
+                    if constexpr (kLate) {
+                        set_rows();
+                        fetch_slice();
+                    }
                     cluster_meet();
                     if constexpr (kEpi) {
                         if (ok && any_rows) finish_slice();
@@ -988,6 +1003,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     // with the three 7.3 and 9.4; gated 2048 x 4096 x 1024 28.8 and 35.1, to codes 30.6 and 34.8 (with both outputs in one kernel, which
                     // spills in its main loop, 32.8 and 34.7).
                     if (!ok) break;
+                    if constexpr (kLate) set_rows();
                     const int buf = acc ^ 1;
                     const uint32_t t_buf = tmem_base + lane_addr + buf * BN + grp * (kGated ? 64 : COLS_PER_GROUP);
 #pragma unroll
