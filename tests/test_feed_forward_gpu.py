@@ -6,7 +6,8 @@ Tolerances, from the arithmetic:
   * a GEMM value: the tensor core adds K/32 products of 32 exact terms and the block-scale promotion K/128 scaled partials, each in
     fp32 with at most one unit of the last place (2^-23) of what has been summed, so at most (K/32 + 2 K/128 + 8) * 2^-23 of the sum
     of absolute products (scales and bias multiplied in are the 8);
-  * an activation has a slope of at most 1.13 and is evaluated to 2^-19 of its value;
+  * an activation has a slope of at most 1.13 and is evaluated to 2^-19 of its value; from -3 down the forms of gelu, from -20 silu, to
+    2^-15.7 (the exponent's rounding), but there the value is under 2^-9 |v|, so that error is under the 8 * 2^-23 |v| of the GEMM's;
   * RMSNorm: at most 136 additions per statistic (128 in a thread, 8 across lanes and warps), half of that through the square root,
     and four roundings: 2^-16 of the value.
 Codes are held to the interval that the value's tolerance leaves: e4m3((y - tol) / s) <= code <= e4m3((y + tol) / s)."""
