@@ -1321,8 +1321,8 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
             }
         }
         // Whole waves, then the tiles that are left in a launch of their own, split.  That launch costs about 10 us from the end of the one
-        // ahead of it to its own, so K has to be long: one launch / two, us, 4096 x 4096 x 14336 269 / 253, 2048 x 8192 x 8192 164 / 158, but
-        // 4096 x 14336 x 4096 291 / 297, 1024 x 14336 x 4096 82.8 / 84.6.
+        // ahead of it to its own, so K has to be long: one launch / two, us, 4096 x 4096 x 14336 268 / 252, 2048 x 8192 x 8192 158 / 149,
+        // 1024 x 14336 x 4096 89.7 / 83.5, but 4096 x 14336 x 4096 283 / 284, gated 1024 x 14336 x 4096 136 / 136.5.
         const int64_t left = tiles % sms;
         for (int split = 2; tails && waves > 1 && left && split <= 8 && split <= kblocks && left * split <= sms; split *= 2) {
             const double us = (waves - 1) * (kblocks * c.full_us + c.wave_us) + (kblocks + split - 1) / split * c.full_us * 1.15 + c.wave_us + c.split_us + 0.3 * split + 10;
@@ -1336,9 +1336,9 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
     return best;
 }
 
-// Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 8.7 / 9.6 / 9.3,
-// 10.5 / 11.9 / 11.6; x 2048 12.8 / 11.8 / 10.2, 16.2 / 14.8 / 12.9; x 14336 49.0 / 32.4 / 21.9, 70.4 / 42.0 / 28.1; 128 x 1024 x 8192
-// 29.8 / 20.9 / 13.9 (11.0), 40.1 / 26.5 / 18.1 (15.7); 512 x 4096 x 4096 19.9, 25.6 / 21.0; 300 x 14336 x 4096 52.5, 50.1.
+// Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 6.8 / 9.5 / 9.3,
+// 9.2 / 11.8 / 10.6; x 2048 10.8 / 11.5 / 10.2, 14.9 / 14.7 / 12.1; x 14336 46.6 / 31.1 / 21.9, 67.3 / 41.4 / 27.1; 128 x 1024 x 8192
+// 28.0 / 20.0 / 13.5 (10.8), 39.4 / 26.2 / 17.6 (14.4); 512 x 4096 x 4096 17.8, 24.5 / 21.1; 300 x 14336 x 4096 46.9, 46.8.
 template <int kOut>
 TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool wide_ok) {
     const void* narrow = nullptr;          // FP8 output: a tile has to hold whole scale groups
