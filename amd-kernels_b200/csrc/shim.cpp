@@ -24,10 +24,10 @@ namespace {
 
 // A tensor's extents, in place: a vector per argument is an allocation per argument.
 struct Shape {
-    int64_t d[8];
+    int64_t d[64];             // as many dimensions as a tensor can have
     int n = 0;
     void push_back(int64_t v) {
-        if (n == 8) fail("tensors of more than 8 dimensions are not accepted");
+        if (n == 64) fail("tensor has too many dimensions");
         d[n++] = v;
     }
     int size() const { return n; }

@@ -166,3 +166,12 @@ def test_gated_checks_its_tensors(hk):
     call("c_scale must be", c_scale=torch.zeros(4, 2))
     call("c_scale: dtype", c_scale=bf(4, 1))
     call("same K", A=f8(4, 128))
+
+
+def test_many_leading_dimensions_are_a_batch(hk):
+    ones = (1,) * 10
+    a, b = torch.zeros(*ones, 4, 128, dtype=E4M3), torch.zeros(*ones, 256, 128, dtype=E4M3)
+    c, sa, sb = torch.zeros(*ones, 4, 256, dtype=torch.bfloat16), torch.ones(*ones, 4), torch.ones(*ones, 256)
+    for call in (lambda: hk.gemm.a8w8_per_token.dispatch(a, b, c, sa, sb), lambda: hk.gemm.a8w8_per_token.dispatch_epilogue(a, b, c, sa, sb)):
+        with pytest.raises(RuntimeError, match="CUDA"):         # all that is wrong with them is where they are
+            call()
