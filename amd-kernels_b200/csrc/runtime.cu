@@ -57,7 +57,7 @@ int sm_count() {
 
 int max_clusters(const void* kern, int threads, int smem, int cluster) {
     struct Entry { int dev; const void* kern; int cluster, n; };
-    static Entry table[64];
+    static Entry table[512];
     static int used = 0;
     int dev = 0;
     if (current_device(&dev) != HKB_OK) return 0;
