@@ -283,18 +283,18 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* crow, int col0, int N
     }
 }
 
-// Groups of four epilogue warps, each with its share of a tile's columns.  Block scales with an epilogue of their own have two for a
-// 128-wide tile as well: one warp alone on its scheduler hides nothing of the tensor memory's latency.  One and two groups, us:
-// 70 x 4096 x 2048 8.9 / 8.0, 300 x 1024 x 8192 13.7 / 12.6, 70 x 4096 x 1024 with bias, gelu and residual 8.8 / 8.3, gated (F = 512)
-// 70 x 512 x 8192 9.3 / 8.5; no size tried was more than 0.2 behind.
-template <int BN, bool kBlockScale, bool kGn128 = false, int kOut = 0>
-constexpr int epi_groups() { return BN == 256 || (kBlockScale && kGn128 && kOut >= 5) ? 2 : 1; }
+// Groups of four epilogue warps, each with its share of a tile's columns.  Block scales, K split: two for a 128-wide tile as well, since
+// one warp alone on its scheduler hides nothing of the tensor memory's latency.  One and two groups, us: 70 x 4096 x 2048 8.9 / 8.0,
+// 300 x 1024 x 8192 13.7 / 12.6, 70 x 4096 x 14336 20.0 / 18.4, gated (F = 512) 70 x 512 x 8192 9.3 / 8.5.  Tiles with the whole of K keep
+// one: they gain where K is short (70 x 4096 x 1024 6.6 / 6.3) and lose where it is not (300 x 4096 x 4096 15.7 / 16.9).
+template <int BN, bool kBlockScale, bool kSplitK = false>
+constexpr int epi_groups() { return BN == 256 || (kBlockScale && kSplitK) ? 2 : 1; }
 // K blocks whose scales are staged at a time: fewer where the room is needed (a 128-wide tile with two groups: for its fifth operand
-// stage, without which 70 x 14336 x 4096 takes 18.1 us for 17.4).
-template <int BN, int kOut>
-constexpr int scale_chunk() { return kOut == 1 ? 16 : BN == 128 && kOut >= 5 ? 16 : 32; }
-template <int BN, bool kBlockScale, bool kPair = false, bool kGn128 = false, int kOut = 0>
-constexpr int gemm_threads() { return ((kBlockScale || kPair) ? 128 : 64) + 128 * epi_groups<BN, kBlockScale, kGn128, kOut>(); }
+// stage, worth 5 % on a K of 14336).
+template <int BN, bool kBlockScale, int kOut, bool kSplitK>
+constexpr int scale_chunk() { return kOut == 1 || (BN == 128 && kBlockScale && kSplitK) ? 16 : 32; }
+template <int BN, bool kBlockScale, bool kPair = false, bool kSplitK = false>
+constexpr int gemm_threads() { return ((kBlockScale || kPair) ? 128 : 64) + 128 * epi_groups<BN, kBlockScale, kSplitK>(); }
 
 __device__ __forceinline__ float2 ffma2(uint32_t a0, uint32_t a1, float2 s, float2 c) {
     return __ffma2_rn(make_float2(__uint_as_float(a0), __uint_as_float(a1)), s, c);
@@ -322,11 +322,11 @@ constexpr int stage_out_bytes() { return kOut == 1 ? (BN == 256 ? 8 : 4) * 4096 
 // warp of every CTA has a share of the epilogue.  The cluster barriers around that are reached by every thread on every path, an
 // abandoned wait included.  A template of its own: the same loop with the part's bounds in variables ran 4-6 % slower whole.
 template <int BN, int STAGES, bool kBlockScale, bool kGn128, bool kPair = false, int AROWS = BM, int kOut = 0, bool kSplitK = false>
-__global__ void __launch_bounds__(gemm_threads<BN, kBlockScale, kPair, kGn128, kOut>(), 1)
+__global__ void __launch_bounds__(gemm_threads<BN, kBlockScale, kPair, kSplitK>(), 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p,
                 const __grid_constant__ CUtensorMap tmBHalf) {
-    constexpr int EPI_GROUPS = epi_groups<BN, kBlockScale, kGn128, kOut>();     // groups of 4 warps; each owns BN/EPI_GROUPS columns
-    constexpr int kScaleChunk = scale_chunk<BN, kOut>();
+    constexpr int EPI_GROUPS = epi_groups<BN, kBlockScale, kSplitK>();     // groups of 4 warps; each owns BN/EPI_GROUPS columns
+    constexpr int kScaleChunk = scale_chunk<BN, kBlockScale, kOut, kSplitK>();
     constexpr int kStageOut = stage_out_bytes<BN, kOut>();
     using L = SmemLayout<BN, STAGES, kPair, AROWS, (kBlockScale && kGn128) ? 128 * EPI_GROUPS : 0, kScaleChunk, kStageOut>;
     constexpr bool kGrouped = kOut == 3;
@@ -334,8 +334,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     static_assert(!kSplitK || EPI_GROUPS * 4 * (BN / EPI_GROUPS) * 128 + (kOut == 7 ? 8 * 8 * 32 * 4 : 0) <= STAGES * L::kStageBytes, "split K: slots in the operand ring");
     constexpr bool kEpi = kOut == 5;
     // With 128 sums and a partial product in its registers the main loop has none to spare, and spills, even outside its steps, cost a
-    // tile about 0.5 us.  So the rows' addresses and the bias are worked out and fetched behind it: 4096 x 4096 x 1024 32.0 and 33.3 us,
-    // 1000 x 14336 x 4096 74.5 and 77.3.
+    // tile about 0.5 us.  So the rows' addresses and the bias are worked out and fetched behind it, and a narrow tile stages its
+    // scales in a rolled loop: 4096 x 4096 x 1024 32.0 and 33.3 us, 1000 x 14336 x 4096 74.5 and 77.3, gated (F = 2048) 300 x 2048 x 1024
+    // 6.8 and 7.6.
     constexpr bool kLate = kEpi && kBlockScale && kGn128;
     constexpr bool kGated = kOut == 6 || kOut == 7, kCodes = kOut == 7;
     static_assert(!kCodes || BN == 256, "FP8 output: a tile is one scale group per row");
@@ -597,7 +598,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const float* src = p.sa + (int64_t)r * all_kblocks + k_begin + kb0;
             const uint32_t dst = smem_u32(sa_slots + (size_t)buf * (kScaleChunk / 4) * EPI_THREADS);
             const bool vec = (kblocks % 4) == 0 && (k_begin % 4) == 0 && (all_kblocks % 4) == 0 && (reinterpret_cast<uintptr_t>(p.sa) & 15) == 0;
-#pragma unroll
+#pragma unroll (kOut >= 5 && BN == 128 ? 2 : 8)
             for (int j = 0; j < kScaleChunk / 4; ++j) {
                 const int kb = kb0 + 4 * j;
                 const uint32_t d = dst + (uint32_t)j * EPI_THREADS * 16;
@@ -842,7 +843,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 // one scale per (row, K block) and per (K block, 128 columns): a single fp32 factor
                 // per thread and K block.  128 accumulators per thread as 64 float2 (packed FMA).
                 constexpr int kHalf = COLS_PER_GROUP / 2;
-                static_assert(COLS_PER_GROUP == 128 || (COLS_PER_GROUP == 64 && kOut >= 5), "block-scale epilogue groups own 128 columns or 64");
+                static_assert(COLS_PER_GROUP == 128 || (COLS_PER_GROUP == 64 && kSplitK), "block-scale epilogue groups own 128 columns or 64");
                 float2 acc2[kHalf];
 #pragma unroll
                 for (int j = 0; j < kHalf; ++j) acc2[j] = make_float2(0.0f, 0.0f);
@@ -1297,7 +1298,7 @@ inline bool skinny_enabled() {
 
 template <int BN, int STAGES, bool kBlockScale, bool kGn128 = false, int AROWS = BM, int kOut = 0, bool kSplitK = false>
 int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p, cudaStream_t st) {
-    using L = SmemLayout<BN, STAGES, false, AROWS, (kBlockScale && kGn128) ? 128 * epi_groups<BN, kBlockScale, kGn128, kOut>() : 0, scale_chunk<BN, kOut>(), stage_out_bytes<BN, kOut>()>;
+    using L = SmemLayout<BN, STAGES, false, AROWS, (kBlockScale && kGn128) ? 128 * epi_groups<BN, kBlockScale, kSplitK>() : 0, scale_chunk<BN, kBlockScale, kOut, kSplitK>(), stage_out_bytes<BN, kOut>()>;
     static_assert(L::kDynamic <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
     auto kern = gemm_fp8_kernel<BN, STAGES, kBlockScale, kGn128, false, AROWS, kOut, kSplitK>;
     // the attribute is per device; set it on every call (cheap) so multi-device processes work
@@ -1306,7 +1307,7 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
     const int sms = sm_count();
     HKB_REQUIRE(sms > 0, HKB_ERR_CUDA, "no CUDA device");
     const int grid = kSplitK ? tiles * p.split : tiles < sms ? tiles : sms;
-    HKB_CUDA(launch_dependent(starts_early(tiles, grid), kern, grid, gemm_threads<BN, kBlockScale, false, kGn128, kOut>(), L::kDynamic, kSplitK ? p.split : 0, st, tmA, tmB, p, tmB));
+    HKB_CUDA(launch_dependent(starts_early(tiles, grid), kern, grid, gemm_threads<BN, kBlockScale, false, kSplitK>(), L::kDynamic, kSplitK ? p.split : 0, st, tmA, tmB, p, tmB));
     if (kSplitK)
         note_kernel(kOut == 5 ? (kBlockScale ? (BN == 256 ? "gemm_fp8_kernel<256,blockscale,epilogue,split>" : "gemm_fp8_kernel<128,blockscale,epilogue,split>")
                                              : (BN == 128 ? "gemm_fp8_kernel<128,pts,epilogue,split>" : "gemm_fp8_kernel<64,pts,epilogue,split>"))
@@ -1367,17 +1368,16 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
     return best;
 }
 
-constexpr int kNarrowStages = 5;         // operand stages of the 128-wide block-scale tiles with an epilogue
 // Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 6.8 / 9.5 / 9.3,
 // 9.2 / 11.8 / 10.6; x 2048 10.8 / 11.5 / 10.2, 14.9 / 14.7 / 12.1; x 14336 46.6 / 31.1 / 21.9, 67.3 / 41.4 / 27.1; 128 x 1024 x 8192
 // 28.0 / 20.0 / 13.5 (10.8), 39.4 / 26.2 / 17.6 (14.4); 512 x 4096 x 4096 17.8, 24.5 / 21.1; 300 x 14336 x 4096 46.9, 46.8.
 template <int kOut>
 TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool wide_ok) {
     const void* narrow = nullptr;          // FP8 output: a tile has to hold whole scale groups
-    if constexpr (kOut != 7) narrow = (const void*)gemm_fp8_kernel<128, kNarrowStages, true, true, false, BM, kOut, true>;
+    if constexpr (kOut != 7) narrow = (const void*)gemm_fp8_kernel<128, 5, true, true, false, BM, kOut, true>;
     const TileCost costs[2] = {
-        {narrow ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, narrow, gemm_threads<128, true, false, true, kOut>(),
-         SmemLayout<128, kNarrowStages, false, BM, 256, scale_chunk<128, kOut>(), stage_out_bytes<128, kOut>()>::kDynamic},
+        {narrow ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, narrow, gemm_threads<128, true, false, true>(),
+         SmemLayout<128, 5, false, BM, 256, scale_chunk<128, true, kOut, true>(), stage_out_bytes<128, kOut>()>::kDynamic},
         {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 2, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
          SmemLayout<256, 3, false, BM, 256, 32, stage_out_bytes<256, kOut>()>::kDynamic}};
     return plan_tiles(costs, M, N, K, 1, true);
@@ -1767,7 +1767,7 @@ int gemm_fp8_blockscale_impl(const void* A, const void* B, void* C, const float*
         return launch_gemm<128, 5, true, true, BM, 1>(tmA, tmB, p, st);
     }
     if (ep) {
-        if (gn == 128) return bn == 256 ? launch_block_scale<256, 3, 5>(tmA, tmB, p, plan, st) : launch_block_scale<128, kNarrowStages, 5>(tmA, tmB, p, plan, st);
+        if (gn == 128) return bn == 256 ? launch_block_scale<256, 3, 5>(tmA, tmB, p, plan, st) : launch_block_scale<128, 5, 5>(tmA, tmB, p, plan, st);
         p.tile_end = p.m_blks * p.n_blks;
         return launch_gemm<128, 6, true, false, BM, 5>(tmA, tmB, p, st);
     }
@@ -1841,7 +1841,7 @@ int hkb_gemm_fp8_blockscale_gated(const void* A, const void* B, void* C, float* 
     rc = make_tmap_bytes(&tmB, B, (uint64_t)K, (uint64_t)(2 * F), 1, (uint32_t)bn / 2);
     if (rc != HKB_OK) return rc;
     if (c_scale) return launch_block_scale<256, 3, 7>(tmA, tmB, p, plan, st);
-    return bn == 256 ? launch_block_scale<256, 3, 6>(tmA, tmB, p, plan, st) : launch_block_scale<128, kNarrowStages, 6>(tmA, tmB, p, plan, st);
+    return bn == 256 ? launch_block_scale<256, 3, 6>(tmA, tmB, p, plan, st) : launch_block_scale<128, 5, 6>(tmA, tmB, p, plan, st);
 }
 
 }  // extern "C"
