@@ -1328,10 +1328,10 @@ int launch_gemm(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams
 // Tile width and CTAs per tile of the kernels with an epilogue of their own (kOut 5, 6, 7).  All tiles take the same time, so what counts
 // is waves x (K blocks per CTA x the time of one, which grows with the share of the SMs at work), at least the time of the epilogue
 // (per-token: it runs beside the next tile's main loop) or plus it (block scales: the accumulators are in its registers); what a wider
-// tile adds once, at the end; and for a split its barriers and exchange and a sixth on every K block.  The weights cannot come faster
+// tile adds once, at the end; and for a split its barriers and exchange and, per-token, a sixth on every K block.  The weights cannot come faster
 // than 5 TB/s.  The constants are fits of the figures at the two callers below.
 struct TilePlan { int bn, split, tail; };          // tail: CTAs per tile of the last, partial wave (1: as the others)
-struct TileCost { int bn; double lone_us, full_us, least_us, wave_us, once_us, split_us; const void* split_kernel; int threads, smem; };
+struct TileCost { int bn; double lone_us, full_us, least_us, wave_us, once_us, split_us, split_factor; const void* split_kernel; int threads, smem; };
 template <int kN>
 TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K, int64_t batch, bool tails, double* us_out = nullptr) {
     const int64_t sms = sm_count(), kblocks = K / BK;
@@ -1344,7 +1344,7 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
         for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
             if (split > 1 && (!c.split_kernel || tiles * split > sms)) break;
             const double busy = tiles * split < sms ? (double)(tiles * split) / sms : 1.0;
-            const double loop = (kblocks + split - 1) / split * (c.lone_us + (c.full_us - c.lone_us) * busy) * (split > 1 ? 1.15 : 1.0);
+            const double loop = (kblocks + split - 1) / split * (c.lone_us + (c.full_us - c.lone_us) * busy) * (split > 1 ? c.split_factor : 1.0);
             double us = waves * (loop > c.least_us ? loop : c.least_us);
             us = (us > stream_us ? us : stream_us) + waves * c.wave_us + c.once_us + (split > 1 ? c.split_us + 0.3 * split : 0);
             if (us < best_us && (split == 1 || tiles <= max_clusters(c.split_kernel, c.threads, c.smem, split))) {
@@ -1368,17 +1368,18 @@ TilePlan plan_tiles(const TileCost (&costs)[kN], int64_t M, int64_t N, int64_t K
     return best;
 }
 
-// Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 6.8 / 9.5 / 9.3,
-// 9.2 / 11.8 / 10.6; x 2048 10.8 / 11.5 / 10.2, 14.9 / 14.7 / 12.1; x 14336 46.6 / 31.1 / 21.9, 67.3 / 41.4 / 27.1; 128 x 1024 x 8192
-// 28.0 / 20.0 / 13.5 (10.8), 39.4 / 26.2 / 17.6 (14.4); 512 x 4096 x 4096 17.8, 24.5 / 21.1; 300 x 14336 x 4096 46.9, 46.8.
+// Block scales.  128-wide whole / in 2 / in 4 (in 8), 256-wide the same, us, with bias and residual: 128 x 4096 x 512 6.8 / 8.0 / 8.1,
+// 9.1 / 11.7 / 10.6; x 2048 10.8 / 10.1 / 9.1, 14.9 / 14.7 / 12.1; x 14336 46.6 / 29.1 / 20.1, 67.0 / 41.2 / 27.0; 128 x 1024 x 8192
+// 28.0 / 18.6 / 12.6 (9.9), 39.3 / 26.3 / 17.6 (14.4); 512 x 4096 x 4096 17.8, 24.5 / 20.5; 300 x 14336 x 4096 46.9, 47.1; without them
+// 1000 x 1024 x 4096 16.7 / 12.8, 21.3 / 17.3 / 15.2.
 template <int kOut>
 TilePlan plan_block_scale(int64_t M, int64_t N, int64_t K, bool wide_ok) {
     const void* narrow = nullptr;          // FP8 output: a tile has to hold whole scale groups
     if constexpr (kOut != 7) narrow = (const void*)gemm_fp8_kernel<128, 5, true, true, false, BM, kOut, true>;
     const TileCost costs[2] = {
-        {narrow ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, narrow, gemm_threads<128, true, false, true>(),
+        {narrow ? 128 : 0, 0.36, 0.46, 0, 1, 0, 1.2, 1.0, narrow, gemm_threads<128, true, false, true>(),
          SmemLayout<128, 5, false, BM, 256, scale_chunk<128, true, kOut, true>(), stage_out_bytes<128, kOut>()>::kDynamic},
-        {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 2, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
+        {wide_ok ? 256 : 0, 0.54, 0.64, 0, 2, 0, 3, 1.0, (const void*)gemm_fp8_kernel<256, 3, true, true, false, BM, kOut, true>, gemm_threads<256, true>(),
          SmemLayout<256, 3, false, BM, 256, 32, stage_out_bytes<256, kOut>()>::kDynamic}};
     return plan_tiles(costs, M, N, K, 1, true);
 }
@@ -1494,9 +1495,9 @@ int launch_pts_epilogue(const void* A, const void* B, GemmParams p, cudaStream_t
                                                   : (const void*)gemm_fp8_kernel<64, 8, false, false, false, BM, 5, true>;
     const int narrow_smem = p.a_box_rows <= 16 ? SmemLayout<64, 19, false, 16>::kDynamic : p.a_box_rows <= 64 ? SmemLayout<64, 12, false, 64>::kDynamic
                                                                                                             : SmemLayout<64, 8>::kDynamic;
-    const TileCost costs[3] = {{64, 0.18, 0.19, 2, 0, 0, 1.8, narrow, gemm_threads<64, false>(), narrow_smem},
-                               {128, 0.22, 0.255, 3, 0, 1, 2.5, (const void*)gemm_fp8_kernel<128, 6, false, false, false, BM, 5, true>, gemm_threads<128, false>(), SmemLayout<128, 6>::kDynamic},
-                               {256, 0.36, 0.413, 4.5, 0, 2.8, 0, nullptr, 0, 0}};      // not split: behind a narrower tile at every size tried
+    const TileCost costs[3] = {{64, 0.18, 0.19, 2, 0, 0, 1.8, 1.15, narrow, gemm_threads<64, false>(), narrow_smem},
+                               {128, 0.22, 0.255, 3, 0, 1, 2.5, 1.15, (const void*)gemm_fp8_kernel<128, 6, false, false, false, BM, 5, true>, gemm_threads<128, false>(), SmemLayout<128, 6>::kDynamic},
+                               {256, 0.36, 0.413, 4.5, 0, 2.8, 0, 1, nullptr, 0, 0}};      // not split: behind a narrower tile at every size tried
     double us = 0;
     const TilePlan plan = plan_tiles(costs, M, N, K, batch, false, &us);
     // CTA pairs take 256 x 256 tiles, the last wave in halves where that is enough (launch_gemm_pair).  64 / 128 / 256-wide tiles / pairs,
