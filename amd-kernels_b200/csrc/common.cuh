@@ -49,12 +49,18 @@ inline int check_launch(const char* what) {
 // visible; that also keeps the chain whole when the next kernel is launched this way in turn.  Only an L2 prefetch, which
 // hands no value to the kernel, may come before it (tma_prefetch_3d).  cluster: CTAs per cluster, 0 = none.
 // early = false: an ordinary launch of the same kernel.
+//
+// Tensor memory is allocated without a limit to the wait, and a CTA of a cluster keeps its own while it waits, without one either, for
+// the rest of its cluster.  Were two such CTAs on one SM, one could wait for the other's memory and the other, at the barrier, for it:
+// of one cluster, or of two clusters that meet on two SMs.  So every CTA of a cluster asks for more than half of an SM's shared memory.
+constexpr size_t kAloneSmem = 114 * 1024;              // of the SM's 228 KB, 1 KB per CTA being the system's
+static_assert(2 * (kAloneSmem + 1024) > 228 * 1024, "two CTAs would fit on an SM");
 template <typename... KArgs, typename... Args>
 cudaError_t launch_dependent(bool early, void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, unsigned cluster, cudaStream_t st, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = cluster > 1 && smem < kAloneSmem ? kAloneSmem : smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;

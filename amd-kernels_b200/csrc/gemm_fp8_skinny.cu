@@ -26,8 +26,10 @@
 // rows >= M, which are never stored (a 16 KB tail pad keeps the overrun of the last stage inside
 // the allocation).  Stage size and stage count are run-time values.
 //
-// Roles, bounded waits and teardown as in gemm_fp8.cu: warp 0 TMA producer, warp 1 TMEM
-// allocator + MMA issuer, warps 2-5 epilogue (two TMEM accumulators of 256 columns).
+// Roles, bounded mbarrier waits and teardown as in gemm_fp8.cu: warp 0 TMA producer, warp 1 TMEM
+// allocator + MMA issuer, warps 2-5 epilogue (two TMEM accumulators of 256 columns).  The TMEM
+// allocation and, where K is split, the cluster barriers have no limit: launch_dependent() keeps
+// the CTAs of clusters on SMs of their own (a ring of narrow tiles, 92 KB, would leave room for two).
 #include "activation.cuh"
 #include "tc_common.cuh"
 
