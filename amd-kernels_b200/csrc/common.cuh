@@ -122,7 +122,9 @@ uint32_t* static_status_peek();
 // ---- device helpers -----------------------------------------------------------------------
 namespace hkb {
 
-// See launch_dependent().  pdl_trigger: the kernel behind this one may be launched once every block has come this far.
+// See launch_dependent().  pdl_trigger: the kernel behind this one may be launched once every block has come this far.  A kernel that
+// allocates tensor memory calls it behind the barrier that follows the allocation: a block of the next kernel keeps what it allocates
+// until this kernel has ended, which it never would with one of its own blocks still waiting for that memory.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

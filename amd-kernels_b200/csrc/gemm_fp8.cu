@@ -417,9 +417,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         else tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
     }
     pdl_wait();      // nothing in global memory is touched before this
-    if (kRange && p.more) pdl_trigger();       // the launch behind this one sets up while this one computes
     tc_fence_before();
     __syncthreads();
+    if (kRange && p.more) pdl_trigger();       // the launch behind this one sets up while this one computes
     if constexpr (kPair) { __syncwarp(); cluster_sync_all(); }   // the partner's barriers and TMEM exist before anyone signals them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;

@@ -120,12 +120,12 @@ gemm_fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         for (int i = 0; i < min(p.stages, kblocks); ++i) tma_prefetch_3d(tile0 < p.rem ? &tmB1 : &tmB0, (k_begin + (kb0 + i) % kblocks) * 128, TILE_COL0(tile0), 0);
     __syncwarp();
     pdl_wait();      // nothing in global memory is read or written before this; the prefetch above is a hint to L2 only
+    tc_fence_before();
+    __syncthreads();
     // The launch behind this one sets up while this one computes.  (The tile kernels do not do this: it changes where the next launch's
     // clusters land.  us, not / so: here 4 x 1024 x 1024 4.7 / 3.7, 64 x 14336 x 4096 14.9 / 13.9; tiles 300 x 4096 x 4096 10.4 / 11.0, a
     // gated layer of 128 rows, 4096 and 14336 wide, 53 / 57.)
     if constexpr (kEpi) pdl_trigger();
-    tc_fence_before();
-    __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 

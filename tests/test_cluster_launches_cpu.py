@@ -1,9 +1,12 @@
 """CPU tier: what keeps the clusters' unbounded waits (tensor-memory allocation, cluster barriers) from waiting on one another, read from
 the launches against the stand-in runtime (fake_cudart.c) in a process of its own, this file as the program."""
 import ctypes
+import glob
+import os
+import re
 
 from test_feed_forward_launches_cpu import _run as run_check
-from test_launches_cpu import LAUNCH, Runtime
+from test_launches_cpu import LAUNCH, ROOT, Runtime
 
 import test_feed_forward_launches_cpu as launches
 
@@ -56,6 +59,21 @@ def check_clusters_have_their_sms_alone():
 def test_clusters_have_their_sms_alone(tmp_path, monkeypatch):
     monkeypatch.setattr(launches, "__file__", __file__)
     run_check("check_clusters_have_their_sms_alone", tmp_path, CLUSTERS)
+
+
+def test_no_dependent_launch_before_the_tensor_memory_is_there():
+    """A kernel that lets the next launch start (whose CTAs allocate tensor memory and then wait for this one to end) has its own by
+    then: in the source, a CTA barrier lies between the allocation and the trigger."""
+    both = 0
+    for path in sorted(glob.glob(os.path.join(ROOT, "amd-kernels_b200", "csrc", "*.cu"))):
+        with open(path) as f:
+            code = re.sub(r"//[^\n]*", "", f.read())
+        for body in code.split("__global__")[1:]:
+            alloc, trigger = body.find("tmem_alloc"), body.find("pdl_trigger()")
+            if alloc >= 0 and trigger >= 0:
+                both += 1
+                assert 0 <= body.find("__syncthreads()", alloc) < trigger, (os.path.basename(path), body[:120])
+    assert both == 3
 
 
 if __name__ == "__main__":
