@@ -22,19 +22,21 @@ namespace {
 
 [[noreturn]] void fail(const std::string& m) { throw std::runtime_error(m); }
 
-// A tensor's extents, in place: a vector per argument is an allocation per argument.
+// A tensor's extents, the first eight in place (a vector per argument is an allocation per argument).
 struct Shape {
-    int64_t d[64];             // as many dimensions as a tensor can have
+    int64_t d[8];
+    std::vector<int64_t> more;
     int n = 0;
     void push_back(int64_t v) {
-        if (n == 64) fail("tensor has too many dimensions");
-        d[n++] = v;
+        if (n < 8) d[n] = v;
+        else more.push_back(v);
+        ++n;
     }
     int size() const { return n; }
-    int64_t back() const { return d[n - 1]; }
+    int64_t back() const { return at(n - 1); }
     int64_t at(int i) const {
         if (i < 0 || i >= n) fail("tensor has too few dimensions");
-        return d[i];
+        return i < 8 ? d[i] : more[(size_t)i - 8];
     }
 };
 
