@@ -532,6 +532,15 @@ void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py:
     check(hkb_gemm_fp8_blockscale_epilogue(A.ptr, B.ptr, C.ptr, (const float*)sa.ptr, (const float*)sb.ptr, gn, bias.none ? nullptr : bias.ptr, act,
                                            res.none ? nullptr : res.ptr, d.M, d.N, d.K, L.stream));
 }
+// Device memory for one call.  It is torch's, so that its life follows the stream (or the captured graph) that uses it; `like`, an f32
+// argument of the call, makes it itself where it is a plain tensor, which needs no lookups.
+[[maybe_unused]] py::object workspace(const py::object& like, int64_t bytes, int device) {
+    Torch* const T = torch_cached();
+    PyObject* const type = reinterpret_cast<PyObject*>(Py_TYPE(like.ptr()));
+    if (T && (type == T->tensor || type == T->parameter)) return like.attr("new_empty")((bytes + 3) / 4);
+    py::module_ torch = py::module_::import("torch");
+    return torch.attr("empty")(bytes, py::arg("dtype") = torch.attr("uint8"), py::arg("device") = torch.attr("device")("cuda", device));
+}
 // Not in the reference: gate and up projection (B [2F, K], gate rows first) and act(gate) * up in one GEMM.  C bf16 [M, F], or with
 // c_scale [M, F/128] e4m3fn codes.
 [[maybe_unused]] void dispatch_blockscale_gated(py::object A_, py::object B_, py::object C_, py::object sa_, py::object sb_, py::object cs_,
@@ -554,11 +563,10 @@ void blockscale(py::object A_, py::object B_, py::object C_, py::object sa_, py:
     const int act = activation(act_);
     same_device({&A, &B, &C, &sa, &sb, &cs});
     Launch L(A.device);
-    // the workspace is torch's, so that its life follows the stream (or the captured graph) that uses it
     const int64_t bytes = hkb_gemm_fp8_blockscale_gated_workspace(M, F, K, cs.none ? 0 : 1);
     if (bytes < 0) check((int)bytes);
     py::object ws;
-    if (bytes > 0) ws = cs_.attr("new_empty")(bytes / 4);
+    if (bytes > 0) ws = workspace(cs_, bytes, A.device);
     check(hkb_gemm_fp8_blockscale_gated(A.ptr, B.ptr, C.ptr, cs.none ? nullptr : (float*)cs.ptr, (const float*)sa.ptr, (const float*)sb.ptr, act,
                                         ws ? reinterpret_cast<void*>(ws.attr("data_ptr")().cast<uint64_t>()) : nullptr, M, F, K, L.stream));
 }

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_feed_forward_gpu import DEV, check_linear, linear_case
+from test_feed_forward_gpu import DEV, E4M3, check_linear, gated_case, linear_case
 
 pytestmark = pytest.mark.gpu
 SPLIT = "gemm_fp8_skinny_kernel<epilogue,split>"
@@ -39,3 +39,30 @@ def test_narrow_split_layers_back_to_back_and_on_two_streams(hk):
     for out in outs:
         for got in out:
             assert all(torch.equal(c, case[6]) for c, case in zip(got, cases))
+
+
+class Duck:
+    """What the boundary needs of a tensor, and nothing else."""
+
+    def __init__(self, t):
+        self.shape, self.keep = tuple(t.shape), t
+
+    def data_ptr(self):
+        return self.keep.data_ptr()
+
+
+class Named(torch.Tensor):
+    """A subclass: read through the general path."""
+
+
+@pytest.mark.parametrize("M", [5, 40])
+@pytest.mark.parametrize("wrap", [Duck, lambda t: t.as_subclass(Named)])
+def test_gated_codes_of_other_tensor_types(hk, M, wrap):
+    """Operands that are not plain tensors, with and without a workspace behind the call."""
+    F, K = 256, 256
+    a, b, sa, sb, *_ = gated_case(M, F, K, 3)
+    want = [torch.empty(M, F, dtype=E4M3, device=DEV), torch.empty(M, F // 128, device=DEV)]
+    hk.gemm.a8w8_blockscale.dispatch_gated(a, b, want[0], sa, sb, want[1], "silu")
+    got = [torch.empty_like(t) for t in want]
+    hk.gemm.a8w8_blockscale.dispatch_gated(wrap(a), wrap(b), wrap(got[0]), wrap(sa), wrap(sb), wrap(got[1]), "silu")
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
