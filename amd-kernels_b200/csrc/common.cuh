@@ -227,6 +227,23 @@ struct Divider2 {
     }
 };
 
+// e4m3 codes of y / s for fp32 y no larger than 448 s (s = amax / 448, not below 1e-10).  1/s in two parts, r + low with r rounded
+// down and low = (1 - s r) r (the bracket is exact in an FMA): y r + y low is y / s to 2^-46 (s < 2^100) ahead of its one rounding, so a quotient that
+// lies between two codes exactly is not moved to either side, and with low >= 0 a zero keeps its sign.  An infinite scale has r = low = 0:
+// finite values give 0, infinite ones NaN, as the division does; NaN stays NaN.
+struct CodeDivider {
+    float2 r2, low2;
+    __device__ __forceinline__ explicit CodeDivider(float s) {
+        const float r = __frcp_rd(s), low = s == __int_as_float(0x7F800000) ? 0.0f : __fmaf_rn(-s, r, 1.0f) * r;
+        r2 = make_float2(r, r);
+        low2 = make_float2(low, low);
+    }
+    __device__ __forceinline__ uint32_t operator()(float2 a, float2 b) const {       // four codes, a.x in bits 0-7
+        const float2 p = __ffma2_rn(a, r2, __fmul2_rn(a, low2)), q = __ffma2_rn(b, r2, __fmul2_rn(b, low2));
+        return (uint32_t)cvt_e4m3x2(p.x, p.y) | ((uint32_t)cvt_e4m3x2(q.x, q.y) << 16);
+    }
+};
+
 // max |.| over the 8 bf16 of a chunk as a packed bf16 pair (both halves hold partial maxima)
 __device__ __forceinline__ __nv_bfloat162 amax8_packed(const uint4& v) {
     auto h2 = [](const uint32_t& w) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };

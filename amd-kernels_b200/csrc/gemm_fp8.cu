@@ -970,11 +970,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             cluster_meet();
                             if (mine) {
                                 for (int r = 0; r < split; ++r) am = max_nan(am, max_nan(maxima[(r * EPI_WARPS + ew) * 32 + lane], maxima[(r * EPI_WARPS + (ew ^ 4)) * 32 + lane]));
-                                const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f), rs = __frcp_rn(scale);
+                                const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f);
+                                const CodeDivider codes(scale);
                                 for (int i = 0; i < outs / 8; ++i) {
                                     gated8(i, y);
-                                    const uint2 o = make_uint2((uint32_t)cvt_e4m3x2(y[0] * rs, y[1] * rs) | ((uint32_t)cvt_e4m3x2(y[2] * rs, y[3] * rs) << 16),
-                                                               (uint32_t)cvt_e4m3x2(y[4] * rs, y[5] * rs) | ((uint32_t)cvt_e4m3x2(y[6] * rs, y[7] * rs) << 16));
+                                    const uint2 o = make_uint2(codes(make_float2(y[0], y[1]), make_float2(y[2], y[3])), codes(make_float2(y[4], y[5]), make_float2(y[6], y[7])));
                                     if (row_ok) *reinterpret_cast<uint2*>(p.q_out + (int64_t)row * F + out0 + 8 * i) = o;
                                 }
                                 if (row_ok && grp == 0 && part == 0) p.q_scale[(int64_t)row * (F / 128) + nb] = scale;
@@ -1080,7 +1080,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             if (!__all_sync(0xFFFFFFFFu, mbar_wait(xb, (max_n >> 1) & 1, abort_flag, p.status, kErrWaitEpilogue, p.wait_ns))) { ok = false; break; }
                             am = max_nan(am, slots[(ew ^ 4) * 32 + lane]);
                             ++max_n;
-                            const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f), rs = __frcp_rn(scale);
+                            const float scale = max_nan(__fdiv_rn(am, 448.0f), 1e-10f);
+                            const CodeDivider codes(scale);
 #pragma unroll 1
                             for (int c = 0; c < kHalf; c += 32) {
                                 uint32_t y[32], o[8];
@@ -1088,8 +1089,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                                 tmem_ld_wait();
 #pragma unroll
                                 for (int j = 0; j < 8; ++j)
-                                    o[j] = (uint32_t)cvt_e4m3x2(__uint_as_float(y[4 * j]) * rs, __uint_as_float(y[4 * j + 1]) * rs) |
-                                           ((uint32_t)cvt_e4m3x2(__uint_as_float(y[4 * j + 2]) * rs, __uint_as_float(y[4 * j + 3]) * rs) << 16);
+                                    o[j] = codes(make_float2(__uint_as_float(y[4 * j]), __uint_as_float(y[4 * j + 1])),
+                                                 make_float2(__uint_as_float(y[4 * j + 2]), __uint_as_float(y[4 * j + 3])));
                                 if (row_ok)
                                     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                                                  ::"l"(p.q_out + (int64_t)row * F + out0 + c), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]),

@@ -2,7 +2,7 @@
 //
 //   h = bf16(x + residual)                     the new residual stream, stored
 //   y = h * rsqrt(mean(h^2) + eps) * w         fp32, never stored
-//   scale = max(amax|y| / 448, 1e-10), q = e4m3fn_rne(clamp(y / scale, +-448)), amax over 128 columns or over the row
+//   scale = max(amax|y| / 448, 1e-10), q = e4m3fn_rne(clamp(y / scale, +-448)), amax over 128 columns or over the row (CodeDivider)
 //
 // h is rounded to bf16 before it is normalised, because the stored stream is what every later layer sees: the result is that of
 // an addition into the stream followed by the norm of the stream.  Sums, statistics and y stay in fp32.
@@ -110,7 +110,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
     const float rinv = rsqrtf(ss / (float)p.D + p.eps);
     const float2 rinv2 = make_float2(rinv, rinv);
 
-    // y of chunk i, computed where it is needed: the gain comes from L1 / L2
+    // y of chunk i; the gain comes from L1 / L2
     auto normed = [&](int i, float2 (&y)[EL / 2]) {
         const int c = t + i * team;
         uint4 w[EL / 8];
@@ -126,34 +126,37 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
         }
         return am;
     };
-    // y is defined up to the order of the sum of squares, so the quotient is y * RN(1/scale), within one fp32 ulp of the division.
-    auto emit = [&](int i, const float2 (&y)[EL / 2], float rs) {
+    // The quotient is rounded as a division rounds it.  y * RN(1/scale) is within an fp32 ulp of that, but h and w have few bits, so many
+    // quotients lie between two codes exactly, and that ulp decides them: of 16384 x 8192 codes 11967 were not those of 64 bits, now 10977
+    // (the order of the sum of squares decides the rest).  1000 x 4096 with block scales 4.8 -> 4.9 us, 16384 x 8192 no difference.
+    auto emit = [&](int i, const float2 (&y)[EL / 2], const CodeDivider& codes) {
         const int c = t + i * team;
-        const float2 rs2 = make_float2(rs, rs);
         uint32_t o[EL / 4];
 #pragma unroll
-        for (int j = 0; j < EL / 4; ++j) {
-            const float2 qa = __fmul2_rn(y[2 * j], rs2), qb = __fmul2_rn(y[2 * j + 1], rs2);
-            o[j] = (uint32_t)cvt_e4m3x2(qa.x, qa.y) | ((uint32_t)cvt_e4m3x2(qb.x, qb.y) << 16);
-        }
+        for (int j = 0; j < EL / 4; ++j) o[j] = codes(y[2 * j], y[2 * j + 1]);
         if (live && c < chunks) store_codes(p.q + base + (int64_t)c * EL, o);
     };
 
-    float2 y[EL / 2];
     if constexpr (kRowScale) {
+        // y stays in registers for the second pass instead of h; with 48 of them that costs a CTA of the SM, so there it is computed again.
+        // Again / kept, us: 1000 x 4104 6.4 / 6.0, 2000 x 16384 52.9 / 37.6, 4000 x 32768 155.6 / 153.7; 4000 x 8200 (48) 44.0 / 48.5.
+        constexpr bool kKeep = EL * NW != 48;
+        float2 y[kKeep ? NW : 1][EL / 2];
         float am = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) am = max_nan(am, normed(i, y));
+        for (int i = 0; i < NW; ++i) am = max_nan(am, normed(i, y[kKeep ? i : 0]));
         am = row_reduce(1, am, [](float a, float b) { return max_nan(a, b); });
-        const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor), rs = __frcp_rn(scale);
+        const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor);
+        const CodeDivider codes(scale);
         if (live && t == 0) p.scales[row] = scale;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            normed(i, y);
-            emit(i, y, rs);
+            if constexpr (!kKeep) normed(i, y[0]);
+            emit(i, y[kKeep ? i : 0], codes);
         }
     } else {
         constexpr int LANES = 128 / EL;
+        float2 y[EL / 2];
         float* const sr = p.scales + row * (p.D / 128);
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
@@ -161,7 +164,7 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) am = max_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
             const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor);
-            emit(i, y, __frcp_rn(scale));
+            emit(i, y, CodeDivider(scale));
             const int c = t + i * team;
             if (live && c < chunks && t % LANES == 0) sr[c / LANES] = scale;
         }
@@ -214,12 +217,12 @@ quant_f32_1x128_kernel(const float* __restrict__ y, uint8_t* __restrict__ q, flo
     for (int k = 0; k < 16; ++k) am = max_nan(am, fabsf(v[k]));
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) am = max_nan(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
-    const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor), rs = __frcp_rn(scale);
+    const float scale = max_nan(__fdiv_rn(am, kFp8Max), kScaleFloor);
     if (g < groups) {
+        const CodeDivider codes(scale);
         uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            o[k] = (uint32_t)cvt_e4m3x2(v[4 * k] * rs, v[4 * k + 1] * rs) | ((uint32_t)cvt_e4m3x2(v[4 * k + 2] * rs, v[4 * k + 3] * rs) << 16);
+        for (int k = 0; k < 4; ++k) o[k] = codes(make_float2(v[4 * k], v[4 * k + 1]), make_float2(v[4 * k + 2], v[4 * k + 3]));
         *reinterpret_cast<uint4*>(q + g * 128 + sub * 16) = make_uint4(o[0], o[1], o[2], o[3]);
         if (sub == 0) scales[g] = scale;
     }

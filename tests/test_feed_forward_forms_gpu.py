@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_feed_forward_gpu import DEV, E4M3, check_linear, gated_case, linear_case
+from test_feed_forward_gpu import DEV, E4M3, check_linear, gated_case, gen, linear_case, quant_rows
 
 pytestmark = pytest.mark.gpu
 SPLIT = "gemm_fp8_skinny_kernel<epilogue,split>"
@@ -66,3 +66,51 @@ def test_gated_codes_of_other_tensor_types(hk, M, wrap):
     got = [torch.empty_like(t) for t in want]
     hk.gemm.a8w8_blockscale.dispatch_gated(wrap(a), wrap(b), wrap(got[0]), wrap(sa), wrap(sb), wrap(got[1]), "silu")
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
+
+
+# ---- codes of values that are known exactly: bit for bit those of an IEEE division ------------------------
+
+def same_codes(q, s, y, group):
+    want_q, want_s = quant_rows(y, group)
+    assert torch.equal(s.view_as(want_s), want_s)
+    differ = (q.view(torch.uint8) != want_q.view(torch.uint8)).sum().item()
+    assert differ == 0, f"{differ} of {q.numel()} codes"
+
+
+@pytest.mark.parametrize("offset", [0, 8])                            # 16- and 8-element chunks
+@pytest.mark.parametrize("per_row", [False, True])
+@pytest.mark.parametrize("D", [1024, 4096, 8192, 32768])
+def test_add_norm_codes_of_exact_values(hk, D, per_row, offset):
+    """h = +-1 in every column and eps = 0: the norm is 1 exactly and y = +-w.  Gains of few bits put quotients on the edge between two
+    codes, where a quotient that is one unit off goes to the other side."""
+    g = gen(D + offset)
+    M = 8
+    for bits in (3, 4, 5, 6, 8):
+        w = torch.randint(0, 1 << bits, (D,), generator=g, device=DEV).bfloat16()
+        h = torch.randint(0, 2, (M, D), generator=g, device=DEV) * 2.0 - 1
+        def view(t):                                                  # noqa: E306
+            return torch.empty(M * D + offset, dtype=torch.bfloat16, device=DEV)[offset:].view(M, D).copy_(t)
+        x, r, out = view(0.25 * h), view(0.75 * h), view(torch.zeros_like(h))
+        q, s = torch.empty(M, D, dtype=E4M3, device=DEV), torch.empty(M, 1 if per_row else D // 128, device=DEV)
+        hk.fused_add_rmsnorm_fp8_quant_fwd(x, r, w, q, s, out, 0.0)
+        same_codes(q, s, h * w.float(), D if per_row else 128)
+
+
+@pytest.mark.parametrize("M,F,K,kernel", [(5, 512, 256, "gemm_fp8_blockscale_skinny_kernel<gated>"), (20, 256, 8192, "gemm_fp8_blockscale_skinny_kernel<gated,split>"),
+                                          (200, 512, 256, "gemm_fp8_kernel<256,blockscale,gated>"), (70, 256, 4096, "gemm_fp8_kernel<256,blockscale,gated,split>")])
+def test_gated_codes_of_exact_values(hk, M, F, K, kernel):
+    """gate = 1 without activation, up = a sum of two or three small integers: y is known exactly."""
+    g = gen(M + F + K)
+    a, b = torch.zeros(M, K, device=DEV), torch.zeros(2 * F, K, device=DEV)
+    b[:F, 2] = 1
+    b[F:, 0] = 16.0 * torch.randint(0, 16, (F,), generator=g, device=DEV)
+    b[F:, 1] = torch.randint(-15, 16, (F,), generator=g, device=DEV).float()
+    a[:, 0] = torch.randint(-1, 2, (M,), generator=g, device=DEV).float()
+    a[:, 1] = torch.randint(0, 4, (M,), generator=g, device=DEV).float()
+    a[:, 2] = 1
+    y = a @ b[F:].t()
+    sa, sb = torch.ones(M, K // 128, device=DEV), torch.ones(K // 128, 2 * F // 128, device=DEV)
+    c, cs = torch.empty(M, F, dtype=E4M3, device=DEV), torch.empty(M, F // 128, device=DEV)
+    hk.gemm.a8w8_blockscale.dispatch_gated(a.to(E4M3), b.to(E4M3), c, sa, sb, cs, "none")
+    assert hk.gemm.a8w8_blockscale.hkb_last_kernel() == kernel
+    same_codes(c, cs, y, 128)
