@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_feed_forward_gpu import DEV, E4M3, check_linear, gated_case, gen, linear_case, quant_rows
+from test_feed_forward_gpu import (DEV, E4M3, act64, act_tol, check_bf16, check_linear, check_norm, gated_case, gen, linear_case, norm_case,
+                                   quant_rows)
 
 pytestmark = pytest.mark.gpu
 SPLIT = "gemm_fp8_skinny_kernel<epilogue,split>"
@@ -114,3 +115,93 @@ def test_gated_codes_of_exact_values(hk, M, F, K, kernel):
     hk.gemm.a8w8_blockscale.dispatch_gated(a.to(E4M3), b.to(E4M3), c, sa, sb, cs, "none")
     assert hk.gemm.a8w8_blockscale.hkb_last_kernel() == kernel
     same_codes(c, cs, y, 128)
+
+
+# ---- every norm kernel: chunks of 8 on wide rows, 3, 6 and 8 of them per thread --------------------------------
+
+@pytest.mark.parametrize("M,D", [(3, 4232), (2500, 520), (3, 8200), (40, 12280), (2, 12296)])
+def test_add_norm_row_scales_of_odd_widths(hk, M, D):
+    check_norm(hk, *norm_case(M, D, M + D), D)
+
+
+@pytest.mark.parametrize("per_row", [False, True])
+@pytest.mark.parametrize("M,D", [(5, 128), (3, 4224), (2400, 512), (7, 8192), (3, 16384), (2, 32768)])
+def test_add_norm_on_views_that_start_inside_32_bytes(hk, M, D, per_row):
+    x, r, w = norm_case(M, D, M + D)
+    x, r = (torch.empty(M * D + 8, dtype=torch.bfloat16, device=DEV)[8:].view(M, D).copy_(t) for t in (x, r))
+    check_norm(hk, x, r, w, D if per_row else 128)
+
+
+# ---- split kernels: the residual stream updated in place, operands that start inside 32 bytes -------------------
+
+PTS = "gemm_fp8_kernel<{},pts,epilogue{}>".format
+BLOCK = "gemm_fp8_kernel<{},blockscale,epilogue{}>".format
+BLOCK_DECODE = "gemm_fp8_blockscale_skinny_kernel<epilogue{}>".format
+
+
+@pytest.mark.parametrize("scales,batch,M,N,K,kernel", [
+    ("token", 1, 5, 1024, 8192, SPLIT), ("token", 1, 64, 1040, 4224, SPLIT), ("token", 1, 8, 128, 4096, SPLIT),
+    ("token", 1, 61, 1032, 4224, PTS(64, ",split")), ("token", 2, 40, 520, 4096, PTS(64, ",split")), ("token", 1, 300, 1024, 8192, PTS(128, ",split")),
+    ("block", 1, 9, 2048, 4224, BLOCK_DECODE(",split")), ("block", 1, 32, 1024, 8192, BLOCK_DECODE(",split")),
+    ("block", 1, 300, 128, 5248, BLOCK(128, ",split")), ("block", 1, 600, 1024, 8320, BLOCK(256, ",split")),
+    ("block", 1, 2047, 8192, 8320, BLOCK(256, ",split"))])                          # whole waves and a split rest
+def test_linear_split_in_place(hk, scales, batch, M, N, K, kernel):
+    check_linear(hk, scales, batch, M, N, K, act="silu", in_place=True, kernel=kernel)
+
+
+@pytest.mark.parametrize("scales,batch,M,N,K,kernel", [
+    ("token", 1, 16, 1024, 256, PTS(64, "")), ("token", 1, 60, 1024, 4096, PTS(64, ",split")), ("token", 1, 5, 1024, 8192, PTS(64, ",split")),
+    ("token", 2, 77, 1032, 384, PTS(64, "")), ("token", 1, 2048, 1024, 8192, PTS(128, "")), ("token", 1, 300, 1024, 8192, PTS(128, ",split")),
+    ("token", 1, 1000, 9008, 256, PTS(256, "")), ("token", 1, 4000, 4048, 2048, PTS("256", "").replace("pts", "pts,pair")),
+    ("block", 1, 9, 256, 256, BLOCK_DECODE("")), ("block", 1, 9, 2048, 4224, BLOCK_DECODE(",split")), ("block", 1, 300, 256, 256, BLOCK(128, "")),
+    ("block", 1, 300, 128, 5248, BLOCK(128, ",split")), ("block", 1, 1025, 9728, 1024, BLOCK(256, "")), ("block", 1, 600, 1024, 8320, BLOCK(256, ",split"))])
+def test_linear_views_that_start_inside_32_bytes(hk, scales, batch, M, N, K, kernel):
+    """Residual, bias and (per-token) the result 16-byte but not 32-byte aligned."""
+    a, b, sa, sb, bi, re, v, tol = linear_case(scales, batch, M, N, K, True, True, M + N + K)
+
+    def off(t):
+        return torch.empty(t.numel() + 8, dtype=t.dtype, device=DEV)[8:].view(t.shape).copy_(t)
+    gemm = hk.gemm.a8w8_per_token if scales == "token" else hk.gemm.a8w8_blockscale
+    c = off(re) if scales == "token" else torch.empty_like(re)
+    gemm.dispatch_epilogue(a, b, c, sa, sb, off(bi), "relu", off(re))
+    assert gemm.hkb_last_kernel() == kernel
+    ref = v + bi.double().unsqueeze(-2)
+    tol = tol + (v.abs() + bi.double().abs().unsqueeze(-2)) * 2.0 ** -23
+    ref, tol = act64(ref, "relu"), act_tol(ref, tol, "relu")
+    ref, tol = ref + re.double(), tol + (ref.abs() + re.double().abs()) * 2.0 ** -23
+    check_bf16(c, ref, tol)
+
+
+# ---- activations to the accuracy that they are written for --------------------------------------------------------
+
+@pytest.mark.parametrize("act,low,high", [("silu", -60.0, 60.0), ("gelu", -11.0, 12.0), ("gelu_tanh", -9.0, 12.0)])
+def test_activations_below_the_result_s_rounding(hk, act, low, high):
+    """The residual takes away the leading part: r = -bf16(ref), so the result is the rest, act(v) + r, exact in fp32 (both are within
+    2^-8 of one another) and rounded to bf16.  Of a dense grid, the arguments whose value is within 2^-14 of a bf16: that rounding is
+    under 2^-8 * 2^-14.  Error of the activation relative to its value, in units of 2^-23 (ex2 is good to two units, rcp to one):
+      silu: the exponent's argument |v| log2(e) / 2 rounds twice, which the square doubles: |v|; the square of ex2 4; reciprocal and
+        products 4;
+      gelu_tanh: the same of z = 1.6 v + 0.07 v^3, and z's own five roundings (two of them of constants), each half a unit of |z|: 3 |z| + 8;
+      gelu: the exponent's argument v^2 log2(e) / 4 with three roundings, doubled, 0.75 v^2; ex2 4, the fit 7.3, Horner steps and their
+        argument 6, products 2."""
+    K = N = 128
+    v = torch.linspace(low, high, 1 << 21, dtype=torch.float64, device=DEV).float()
+    ref = act64(v.double(), act)
+    near = ((ref - ref.bfloat16().double()).abs() <= ref.abs() * 2.0 ** -14) & (ref.abs() >= 2.0 ** -100)
+    pick = near.nonzero().flatten()
+    pick = pick[torch.linspace(0, pick.numel() - 1, 32768, dtype=torch.float64, device=DEV).long()]
+    v, ref = v[pick].contiguous(), ref[pick]
+    lead = ref.bfloat16()
+    M = v.numel()
+    a, b = torch.ones(M, K, device=DEV).to(E4M3), torch.eye(N, K, device=DEV).to(E4M3)
+    c = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    res = (-lead)[:, None].expand(M, N).contiguous()
+    hk.gemm.a8w8_per_token.dispatch_epilogue(a, b, c, v, torch.ones(N, device=DEV), None, act, res)
+    assert torch.equal(c, c[:, :1].expand(M, N))
+    w = v.double().abs()
+    units = {"silu": w + 8, "gelu_tanh": 3 * (1.59577 * w + 0.0713549 * w ** 3) + 8, "gelu": 0.75 * w * w + 19.3}[act]
+    rest = ref - lead.double()
+    err = (c[:, 0].double() - rest).abs()
+    bound = units * 2.0 ** -23 * ref.abs()
+    bound = bound + (rest.abs() + bound) * 2.0 ** -8
+    assert (err <= bound).all(), f"{(err > bound).sum().item()} of {M}, worst {(err / bound).max().item():.3g} of the bound"
