@@ -172,10 +172,12 @@ add_rmsnorm_quant_kernel(const AddNormParams p) {
 }
 
 // Chunks per thread.  Few rows, where only latency counts: one, as many warps per row as it takes.  Else 32 elements per thread (24 in
-// 8-element chunks) in teams of up to 16 (8) warps, more only for rows that need it.  us with 1 / 2 / 3 / 4 chunks of 16: 300 x 4096
-// 3.3 / 4.0 / 4.0 / 4.3, 1000 x 5120 8.0 / 8.3 / 9.3 / 9.6, 4096 x 4096 22.5 / 20.8 / 22.4 / 22.2, 4096 x 5120 31.7 / 26.9 / 27.2 / 31.7,
-// 16384 x 8192 144 / 138 / 149 / 141 (only 1000 x 4096 differs: 6.7 / 6.7 / 6.1 / 5.8); with 1 / 2 / 3 / 4 / 6 / 8 chunks of 8: 8000 x 1032
-// 29.7 / 20.3 / 14.3 / 16.2 / 15.0 / 15.2, 8000 x 2056 35.2 / 34.6 / 25.4 / 25.6 / 29.1 / 29.0, 4000 x 16376 - / - / - / 106 / 114 / 77.
+// 8-element chunks) in teams of up to 16 (8) warps, more only for rows that need it.  us in a replayed graph with 1 / 2 / 3 / 4 chunks of
+// 16, block scales: 300 x 4096 3.3 / 3.5 / 3.9 / 4.2, 1000 x 4096 5.4 / 5.1 / 6.8 / 5.4, 1000 x 5120 6.2 / 6.4 / 7.4 / 7.8, 4096 x 4096
+// 22.1 / 18.6 / 21.0 / 20.2, 4096 x 5120 25.7 / 25.5 / 28.5 / 29.8, 16384 x 8192 146 / 137 / 152 / 140; row scales 1000 x 4096 6.0 / 5.1 /
+// 7.6 / 5.2, 16384 x 8192 189 / 136 / 169 / 144.  With 1 / 2 / 3 / 4 / 6 / 8 chunks of 8, row scales: 8000 x 1032 25.5 / 16.0 / 11.5 / 14.0 /
+// 13.4 / 12.5, 8000 x 2056 33.1 / 30.9 / 21.3 / 22.2 / 27.4 / 27.2, 4000 x 16376 - / - / - / 105 / 113 / 77.  4000 x 8200, the narrowest
+// rows with six, would be ahead with fewer: - / - / 40.9 / 40.4 / 44.7 / 42.7.
 template <int EL, bool kRowScale>
 int dispatch_add_norm(AddNormParams p, cudaStream_t st) {
     const int chunks = p.D / EL, most = (chunks + 31) / 32, sms = sm_count();

@@ -124,7 +124,8 @@ int hkb_quant_mxfp4(const void* x, const void* w_or_null, void* codes, void* sca
  * `group` columns: group = 128 (scales f32 [M, D/128], the block-scale GEMM's a_scale; D % 128 == 0) or
  * group = D (scales f32 [M], the per-token GEMM's).  x, residual, residual_out bf16 [M, D]; w bf16 [D]; q u8
  * [M, D].  residual_out may be residual or x itself (the stream updated in place); any other overlap of outputs
- * with inputs is not allowed.  A NaN or an infinity in a row goes into its codes and scales as the formula says.
+ * with inputs is not allowed.  A NaN or an infinity in a row goes into its codes and scales as the formula says.  The
+ * squares are summed in fp32: where a row's sum passes 3.4e38 (values beyond 1e17 or so) its finite values come out as 0.
  * D % 8 == 0, D <= 32768; x, residual, residual_out and w 16-byte, q 8-byte aligned (fast path: D % 16 == 0,
  * x, residual and residual_out 32-byte and q 16-byte aligned).  No counterpart in the reference project, whose
  * fused quantizers take no residual and whose fused_add_rmsnorm does not quantize. */
