@@ -158,7 +158,7 @@ gemm_fp8_blockscale_skinny_kernel(const __grid_constant__ CUtensorMap tmA, const
     pdl_wait();      // nothing in global memory is read or written before this; the prefetch above is a hint to L2 only
     tc_fence_before();
     __syncthreads();
-    if constexpr (kOut != 0) pdl_trigger();  // the launch behind this one sets up while this one computes: 1 x 1024 x 1024 4.5 -> 3.9 us
+    if constexpr (kOut != 0) pdl_trigger();  // the launch behind this one sets up while this one computes: 1 x 1024 x 1024 4.5 -> 4.0 us
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
